@@ -110,6 +110,26 @@ void topk_select(const torch::Tensor& grad, torch::Tensor& err, c10::optional<to
                  int64_t idx_ptr, int64_t val_ptr, int64_t cnt_ptr);
 void topk_reduce(const torch::Tensor& peers, const torch::Tensor& flags, int64_t slot, int64_t epoch, int64_t list_off,
                  int64_t cnt_index, torch::Tensor& red, double scale, int64_t max_blocks, double budget_s);
+std::tuple<torch::Tensor, torch::Tensor> bounds_from_offsets(const torch::Tensor& offsets, int64_t rows,
+                                                             c10::optional<torch::Tensor> start,
+                                                             c10::optional<torch::Tensor> end);
+std::tuple<torch::Tensor, torch::Tensor> bounds_from_ids(const torch::Tensor& ids, int64_t bos,
+                                                         c10::optional<torch::Tensor> start,
+                                                         c10::optional<torch::Tensor> end);
+std::tuple<torch::Tensor, torch::Tensor> packed_attn_fwd(const torch::Tensor& q, const torch::Tensor& k,
+                                                         const torch::Tensor& v, const torch::Tensor& start,
+                                                         const torch::Tensor& end, int64_t window, double scale,
+                                                         c10::optional<torch::Tensor> out,
+                                                         c10::optional<torch::Tensor> lse);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
+    const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& out,
+    const torch::Tensor& lse, const torch::Tensor& dout, const torch::Tensor& start, const torch::Tensor& end,
+    int64_t window, double scale, c10::optional<torch::Tensor> dq, c10::optional<torch::Tensor> dk,
+    c10::optional<torch::Tensor> dv, c10::optional<torch::Tensor> delta);
+std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> distill_topk(
+    const torch::Tensor& logits, const torch::Tensor& ids, const torch::Tensor& teacher,
+    c10::optional<torch::Tensor> targets, double cap, double temperature, double alpha, double scale, bool need_grad,
+    c10::optional<torch::Tensor> grad);
 }  // namespace br
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -161,6 +181,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("lse"), pybind11::arg("dqkv"), pybind11::arg("delta"), pybind11::arg("B"), pybind11::arg("T"),
         pybind11::arg("H"), pybind11::arg("KV"), pybind11::arg("hd"), pybind11::arg("window"),
         pybind11::arg("which") = 0);
+  m.def("bounds_from_offsets", &br::bounds_from_offsets);
+  m.def("bounds_from_ids", &br::bounds_from_ids);
+  m.def("packed_attn_fwd", &br::packed_attn_fwd);
+  m.def("packed_attn_bwd", &br::packed_attn_bwd);
+  m.def("distill_topk", &br::distill_topk);
   m.def("mc_sharpe", &br::mc_sharpe);
   m.def("comm_push", &br::comm_push);
   m.def("comm_signal_peers", &br::comm_signal_peers);
