@@ -11,17 +11,30 @@
 // Key row j is seen by the queries [j, min(j + w, end[j])). Rows of no sequence (empty span) are neither read
 // as keys nor written. Spans are clamped to the rows that exist, so a bad span reads nothing outside.
 //
-// One warp per row and head: a lane holds D / 32 of the row's values in fp32, a score is a warp-wide sum.
+// Forward: tcgen05 tiles of 128 packed rows by 128 packed keys (described at the kernel). A tile may hold the end of
+// one sequence and the start of the next: the tiles are cut by row number, not by sequence, so a batch of
+// short sequences fills them as well as one long sequence does, no work list has to be built, and the sequences
+// appear only as each row's range of keys. A matrix product multiplies hidden keys by a weight of exactly 0,
+// which does nothing unless such a key holds a value that is no number. Keys before the first sequence of a
+// work item are overwritten with zeros in shared memory; what else is foreign to a row is within its own
+// tiles' rows: a row that came out as no number and has such keys is computed alone, from its own keys
+// (fwd_row). That can be the case only within 256 rows of a border, so its cost stays bounded.
+//
+// Row by row (the backward, and the rows that a tile's product spoils): one warp per row and head, a lane holds
+// D / 32 of the row's values in fp32, a score is a warp-wide sum.
 #include <torch/extension.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <atomic>
 #include <string>
 #include <tuple>
+#include <utility>
 
 #include "half_types.cuh"
 #include "status.h"
+#include "tma_host.h"
 
 namespace br {
 namespace {
@@ -87,7 +100,7 @@ __device__ __forceinline__ int queries_of(const PackedParams& p, int j) {
 }
 
 template <typename T, int D>
-__device__ __forceinline__ void fwd_row(const PackedParams& p, int i, int h, int lane) {
+__device__ __noinline__ void fwd_row(const PackedParams& p, int i, int h, int lane) {
   constexpr int E = D / 32;
   const int2 key = keys_of(p, i);
   if (key.y <= key.x) return;
@@ -95,22 +108,31 @@ __device__ __forceinline__ void fwd_row(const PackedParams& p, int i, int h, int
   float q[E], acc[E] = {};
   load_row<T, D>(p.q, i, h, lane, q);
   float m = -INFINITY, l = 0.f;
-  for (int j = key.x; j < key.y; ++j) {
-    float k[E], v[E];
-    load_row<T, D>(p.k, j, g, lane, k);
-    load_row<T, D>(p.v, j, g, lane, v);
-    const float x = dot(q, k) * p.scale_log2;
-    if (x > m) {  // the same in every lane
-      const float a = exp2f(m - x);
-      l *= a;
+  for (int j0 = key.x; j0 < key.y; j0 += 4) {  // four keys at a time: their loads overlap
+    float v[4][E], x[4];
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] *= a;
-      m = x;
+    for (int u = 0; u < 4; ++u) {
+      float k[E];
+      const int j = min(j0 + u, key.y - 1);
+      load_row<T, D>(p.k, j, g, lane, k);
+      load_row<T, D>(p.v, j, g, lane, v[u]);
+      x[u] = dot(q, k) * p.scale_log2;
     }
-    const float w = exp2f(x - (m == -INFINITY ? 0.f : m));  // a score of -inf has weight 0 also before any other
-    l += w;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+    for (int u = 0; u < 4; ++u) {
+      if (j0 + u >= key.y) break;
+      if (x[u] > m) {  // the same in every lane
+        const float a = exp2f(m - x[u]);
+        l *= a;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= a;
+        m = x[u];
+      }
+      const float w = exp2f(x[u] - (m == -INFINITY ? 0.f : m));  // a score of -inf has weight 0 also before any other
+      l += w;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[u][e], acc[e]);
+    }
   }
   const float inv = 1.f / l;
 #pragma unroll
@@ -175,11 +197,6 @@ __device__ __forceinline__ void dkv_row(const PackedParams& p, int j, int g, int
 constexpr int kRowWarps = 8;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32) fwd_rows_kernel(PackedParams p) {
-  const int i = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  if (i < p.N) fwd_row<T, D>(p, i, blockIdx.y, threadIdx.x & 31);
-}
-template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) dq_rows_kernel(PackedParams p) {
   const int i = blockIdx.x * kRowWarps + (threadIdx.x >> 5), h = blockIdx.y, lane = threadIdx.x & 31;
   if (i >= p.N) return;
@@ -194,6 +211,478 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) dkv_rows_kernel(PackedParams p) {
   const int j = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   if (j < p.N) dkv_row<T, D>(p, j, blockIdx.y, threadIdx.x & 31);
+}
+
+// ---------------------------------------------------------------------------------------- forward, tcgen05
+// Persistent, one CTA per SM, 320 threads. A work item is two 128-row query tiles A and B that share their keys: two
+// heads of one kv head over the same rows where the group of query heads is even, else two neighbouring row
+// tiles of one head. The grid has one block per item; a running CTA takes over blocks that have not started
+// (clc_request), so items of uneven cost balance over the SMs without a counter in memory that two launches
+// would share. Items go from the last rows to the first: in a long sequence the late rows cost most.
+//   warp 0     takes items, hands them to the other warps through a two-slot ring, and issues the TMA loads: the
+//              item's two Q tiles, then K and V tiles into rings;
+//   warp 1     issues the MMAs. Per query tile X: S_X = Q_X K_t^T -> TMEM [256X, +128) fp32; P_X, written there by
+//              the softmax warps as 16-bit pairs over S_X, is the A operand of O_X += P_X V_t -> TMEM
+//              [256X + 128, +D). Order at key tile t: PV_A(t) S_A(t+1) PV_B(t) S_B(t+1), so the tensor core
+//              works on one query tile while the other's softmax runs;
+//   warps 2-9  softmax, one query row per thread (2-5 tile A, 6-9 tile B).
+// S_X(t+1) is issued after PV_X(t) and the MMAs of a CTA complete in order, so a softmax warp that sees S_X(t+1) may
+// overwrite P_X and rescale O_X. P is at most 2^8 (the running maximum is only replaced when it grows by more
+// than that) and is rounded to 16 bits for the product (half a step, relative); the row sum l adds the
+// unrounded fp32 values, the maximum, l and O stay in fp32.
+constexpr uint64_t kBudgetNs = 2000000000ull, kDrainNs = 100000000ull;
+constexpr int BT = 128;  // rows of a query tile, keys of a key tile
+constexpr int kAtom = BT * 128;  // 128 rows x 128 bytes, one 128-byte-swizzle atom column of a tile
+
+template <int D>
+struct FwdCfg {
+  static constexpr int kTile = BT * D * 2;
+  static constexpr int kK = D == 128 ? 3 : 4;  // ring depths: K runs one tile ahead of V
+  static constexpr int kV = D == 128 ? 2 : 4;
+  static constexpr int oQ = 0, oK = 2 * kTile, oV = oK + kK * kTile, oBar = oV + kV * kTile;
+  static constexpr int kSmem = oBar + 384 + 1024;
+  static_assert(kSmem <= 232448, "forward shared memory");
+};
+
+struct FwdMaps {
+  CUtensorMap q, k, v;
+  int swap;  // bit 0: q's map has its coordinates as (d, row, head), bit 1: k's, bit 2: v's
+};
+
+__device__ __forceinline__ void load_tile(const CUtensorMap* m, bool swap, uint64_t* bar, uint8_t* dst, int head, int row,
+                                          int atoms, int atom_bytes) {
+  for (int c = 0; c < atoms; ++c)
+    tma_load_3d(m, bar, dst + c * atom_bytes, 64 * c, swap ? row : head, swap ? head : row);
+}
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+struct FwdItem {
+  int h[2], q0[2];  // head and first row of the query tiles A and B
+  int lo[2], hi[2];  // key tiles [lo, hi) of each (empty: no such query tile)
+  int kvh;
+  __device__ bool uses(int x, int t) const { return t >= lo[x] && t < hi[x]; }
+  __device__ int first() const { return hi[1] > lo[1] ? min(lo[0], lo[1]) : lo[0]; }
+  __device__ int last() const { return max(hi[0], hi[1]); }  // one past the last key tile
+};
+
+// where an item's query tiles are; the key ranges follow from the spans (item_keys) or the ring
+__device__ __forceinline__ FwdItem item_rows(int block, int n_blocks, const PackedParams& p) {
+  FwdItem I;
+  const int item = n_blocks - 1 - block;
+  const int group = p.H / p.KV;
+  if (group % 2 == 0) {
+    const int hp = p.H / 2, tile = item / hp;
+    I.h[0] = 2 * (item % hp);
+    I.h[1] = I.h[0] + 1;
+    I.q0[0] = I.q0[1] = tile * BT;
+  } else {
+    I.h[0] = I.h[1] = item % p.H;
+    I.q0[0] = item / p.H * (2 * BT);
+    I.q0[1] = I.q0[0] + BT;
+  }
+  I.kvh = I.h[0] / group;
+  for (int x = 0; x < 2; ++x) {
+    I.hi[x] = I.q0[x] < p.N ? I.q0[x] / BT + 1 : 0;
+    I.lo[x] = 0;
+  }
+  return I;
+}
+// spans never decrease along the rows, so a tile's first row has its first key
+__device__ __forceinline__ void item_keys(FwdItem& I, const PackedParams& p) {
+  for (int x = 0; x < 2; ++x) I.lo[x] = I.hi[x] > 0 ? min(max(keys_of(p, I.q0[x]).x, 0) / BT, I.hi[x] - 1) : 0;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(320, 1) fwd_tc_kernel(const __grid_constant__ FwdMaps maps,
+                                                        const __grid_constant__ PackedParams p, int* status) {
+  using C = FwdCfg<D>;
+  constexpr int kAtoms = D / 64;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
+  uint64_t* q_full = bars + 0;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* s_full = bars + 2;      // [2] per query tile
+  uint64_t* p_full = bars + 4;      // [2]
+  uint64_t* o_done = bars + 6;      // [2]
+  uint64_t* o_empty = bars + 8;     // [2]
+  uint64_t* item_full = bars + 10;  // [2] ring slots
+  uint64_t* item_empty = bars + 12;
+  uint64_t* drain = bars + 14;
+  uint64_t* clc_full = bars + 15;
+  uint64_t* k_full = bars + 16;
+  uint64_t* k_empty = k_full + C::kK;
+  uint64_t* v_full = k_empty + C::kK;
+  uint64_t* v_empty = v_full + C::kV;
+  static_assert(16 + 2 * (C::kK + C::kV) <= 32, "barrier region");
+  volatile int* ring = reinterpret_cast<volatile int*>(bars + 32);  // [2][4]: block (-1: the end), lo of A, lo of B
+  uint8_t* clc_resp = reinterpret_cast<uint8_t*>(bars + 36);      // 16 bytes
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = warp_id();
+  if (device_failed(status)) return;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], 128);
+      mbar_init(&o_done[x], 1);
+      mbar_init(&o_empty[x], 128);
+      mbar_init(&item_full[x], 1);
+      mbar_init(&item_empty[x], 9);  // the MMA thread and one lane of each softmax warp
+    }
+    mbar_init(drain, 1);
+    mbar_init(clc_full, 1);
+    for (int i = 0; i < C::kK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < C::kV; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto fail = [&](int code) {
+    *abort_flag = 1;
+    if (status) atomicCAS(status, 0, code);
+  };
+  auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, kBudgetNs, abort_flag, status); };
+  auto item_of = [&](int slot) {
+    FwdItem I = item_rows(ring[slot * 4], gridDim.x, p);
+    I.lo[0] = ring[slot * 4 + 1];
+    I.lo[1] = ring[slot * 4 + 2];
+    return I;
+  };
+
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&maps.q);
+      tma_prefetch_desc(&maps.k);
+      tma_prefetch_desc(&maps.v);
+      int ik = 0, iv = 0;  // K and V tiles loaded so far (ring positions)
+      int nq = 0, nc = 0;  // Q loads and requests for work
+      int block = blockIdx.x;
+      bool ok = true;
+      for (int n = 0;; ++n) {
+        const int slot = n & 1;
+        if (n >= 2 && !wait(&item_empty[slot], (n - 2) >> 1)) {
+          ok = false;
+          break;
+        }
+        if (block < 0) {
+          ring[slot * 4] = -1;
+          mbar_arrive(&item_full[slot]);
+          break;
+        }
+        FwdItem I = item_rows(block, gridDim.x, p);
+        item_keys(I, p);
+        ring[slot * 4] = block;
+        ring[slot * 4 + 1] = I.lo[0];
+        ring[slot * 4 + 2] = I.lo[1];
+        mbar_arrive(&item_full[slot]);
+        fence_async_smem();  // the last answer has been read before the next one is written over it
+        clc_request(clc_resp, clc_full);
+        ++nc;
+        if (n > 0 && !wait(q_empty, n - 1)) {  // the previous item's score MMAs have read the Q tiles
+          ok = false;
+          break;
+        }
+        const int nx = I.hi[1] > 0 ? 2 : 1;
+        mbar_arrive_expect_tx(q_full, nx * C::kTile);
+        ++nq;
+        for (int x = 0; x < nx; ++x)
+          load_tile(&maps.q, maps.swap & 1, q_full, smem + C::oQ + x * C::kTile, I.h[x], I.q0[x], kAtoms, kAtom);
+        const int t0 = I.first(), t1 = I.last();
+        for (int t = t0; ok && t <= t1; ++t) {  // K(t0), then K(t+1) and V(t) in turn
+          if (t < t1) {
+            const int st = ik % C::kK;
+            if (!wait(&k_empty[st], (ik / C::kK) ^ 1)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&k_full[st], C::kTile);
+            load_tile(&maps.k, maps.swap & 2, &k_full[st], smem + C::oK + st * C::kTile, I.kvh, t * BT, kAtoms, kAtom);
+            ++ik;
+          }
+          if (t > t0) {
+            const int st = iv % C::kV;
+            if (!wait(&v_empty[st], (iv / C::kV) ^ 1)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&v_full[st], C::kTile);
+            load_tile(&maps.v, maps.swap & 4, &v_full[st], smem + C::oV + st * C::kTile, I.kvh, (t - 1) * BT, kAtoms,
+                      kAtom);
+            ++iv;
+          }
+        }
+        if (!ok || !wait(clc_full, n)) {
+          ok = false;
+          break;
+        }
+        block = clc_block(clc_resp);
+      }
+      if (!ok) {
+        fail(kErrTimeoutProducer);
+        // the copies in flight still write to this block's shared memory
+        for (int g = max(0, ik - C::kK); g < ik; ++g) mbar_wait(&k_full[g % C::kK], (g / C::kK) & 1, kDrainNs, nullptr);
+        for (int g = max(0, iv - C::kV); g < iv; ++g) mbar_wait(&v_full[g % C::kV], (g / C::kV) & 1, kDrainNs, nullptr);
+        if (nq > 0) mbar_wait(q_full, (nq - 1) & 1, kDrainNs, nullptr);
+        if (nc > 0) mbar_wait(clc_full, (nc - 1) & 1, kDrainNs, nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = umma_idesc_16<T>(BT, BT, false, false);
+      constexpr uint32_t idesc_o = umma_idesc_16<T>(BT, D, false, true);
+      int kbase = 0, vbase = 0;            // ring positions of the item's first K and V tiles
+      int pc[2] = {0, 0}, oc[2] = {0, 0};  // per query tile: P blocks consumed, items whose O is complete
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const int slot = n & 1;
+        if (!wait(&item_full[slot], n >> 1)) {
+          ok = false;
+          break;
+        }
+        if (ring[slot * 4] < 0) break;
+        const FwdItem I = item_of(slot);
+        mbar_arrive(&item_empty[slot]);
+        const int t0 = I.first(), t1 = I.last();
+        int scores = I.hi[0] - I.lo[0] + I.hi[1] - I.lo[1];  // score products of the item still to issue
+        ok = wait(q_full, n);
+        auto issue_s = [&](int x, int t) -> bool {  // S_X = Q_X K_t^T
+          const int g = kbase + t - t0, st = g % C::kK;
+          if (!wait(&k_full[st], g / C::kK)) return false;
+          tc_fence_after();
+          const uint32_t q_addr = smem_u32(smem + C::oQ + x * C::kTile), k_addr = smem_u32(smem + C::oK + st * C::kTile);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 32;
+            umma_bf16_ss(tmem + x * 256, umma_desc_sw128(q_addr + off, 16, 1024), umma_desc_sw128(k_addr + off, 16, 1024),
+                         idesc_s, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[x]);
+          if (x == 1 || !I.uses(1, t)) umma_commit(&k_empty[st]);  // the tile's last reader
+          if (--scores == 0) umma_commit(q_empty);
+          return true;
+        };
+        auto issue_pv = [&](int x, int t) -> bool {  // O_X += P_X V_t
+          const int g = vbase + t - t0, st = g % C::kV;
+          // the first product of an item overwrites O: the softmax warps have read the previous item's
+          if (t == I.lo[x] && oc[x] > 0 && !wait(&o_empty[x], oc[x] - 1)) return false;
+          if (!wait(&p_full[x], pc[x]) || !wait(&v_full[st], g / C::kV)) return false;
+          ++pc[x];
+          tc_fence_after();
+          const uint32_t v_addr = smem_u32(smem + C::oV + st * C::kTile);
+#pragma unroll
+          for (int kk = 0; kk < BT / 16; ++kk)
+            umma_bf16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, umma_desc_sw128(v_addr + kk * 2048, kAtom, 1024),
+                         idesc_o, (t > I.lo[x] || kk > 0) ? 1u : 0u);
+          if (x == 1 || !I.uses(1, t)) umma_commit(&v_empty[st]);
+          if (t == I.hi[x] - 1) {
+            umma_commit(&o_done[x]);
+            ++oc[x];
+          }
+          return true;
+        };
+        for (int t = t0 - 1; ok && t < t1; ++t) {
+          for (int x = 0; x < 2 && ok; ++x) {
+            if (I.uses(x, t)) ok = issue_pv(x, t);
+            if (ok && I.uses(x, t + 1)) ok = issue_s(x, t + 1);
+          }
+        }
+        kbase += t1 - t0;
+        vbase += t1 - t0;
+      }
+      if (!ok) fail(kErrTimeoutMma);
+      umma_commit(drain);
+      mbar_wait(drain, 0, kDrainNs, nullptr);
+    }
+  } else {
+    const int x = (warp - 2) >> 2, wq = warp & 3, lane = lane_id();
+    const int r = wq * 32 + lane;  // row of the tile = TMEM lane
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16) + x * 256;
+    int sc = 0, oc = 0;  // score blocks consumed and items finished by this query tile
+    int vbase = 0;       // ring position of the item's first V tile
+    for (int n = 0;; ++n) {
+      const int slot = n & 1;
+      if (!mbar_wait_warp(&item_full[slot], (n >> 1) & 1, kBudgetNs, abort_flag, status)) {
+        fail(kErrTimeoutEpilogue);
+        break;
+      }
+      if (ring[slot * 4] < 0) break;
+      int t_lo, t_hi, h, i, t0, z, vfirst = vbase;
+      {
+        const FwdItem I = item_of(slot);
+        t0 = I.first();
+        vbase += I.last() - t0;
+        z = __ldg(p.start + I.q0[0]);  // keys before it are foreign to every row of the item
+        t_lo = x ? I.lo[1] : I.lo[0];
+        t_hi = x ? I.hi[1] : I.hi[0];
+        h = x ? I.h[1] : I.h[0];
+        i = (x ? I.q0[1] : I.q0[0]) + r;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[slot]);
+      const int2 key = i < p.N ? keys_of(p, i) : make_int2(0, 0);
+      // rows of V that this thread clears before the item's first product
+      const bool clears = x == 0 && t_lo == t0 && t0 * BT + r < z;
+      float m_ref = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int t = t_lo; t < t_hi; ++t, ++sc) {
+        if (!mbar_wait_warp(&s_full[x], sc & 1, kBudgetNs, abort_flag, status)) {
+          fail(kErrTimeoutEpilogue);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int k0 = t * BT;
+        uint32_t sr[4][32];  // this row's scores before scaling
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(lane_base + c * 32, sr[c]);
+        tmem_ld_wait();
+        float mx = -INFINITY;
+        if (__all_sync(0xffffffffu, key.x <= k0 && key.y >= k0 + BT)) {
+          // every key of the tile is visible to the warp's rows
+#pragma unroll
+          for (int e = 0; e < BT; ++e) mx = fmaxf(mx, __uint_as_float(sr[e >> 5][e & 31]));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t vis = range_mask32(key.x - k0 - 32 * c, key.y - k0 - 32 * c);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float s = ((vis >> e) & 1u) ? __uint_as_float(sr[c][e]) : -INFINITY;
+              sr[c][e] = __float_as_uint(s);
+              mx = fmaxf(mx, s);
+            }
+          }
+        }
+        mx *= p.scale_log2;
+        // The rescale is decided per row, but tcgen05.ld/st are warp-collective: the warp rescales together
+        // when any of its rows needs it, the others by 1.
+        float alpha = 1.f;
+        bool mine = false;
+        if (t == t_lo) {
+          m_ref = mx;
+        } else if (mx > m_ref + 8.f) {
+          mine = true;
+          alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
+          l *= alpha;
+          m_ref = mx;
+        }
+        if (__any_sync(0xffffffffu, mine)) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld32(lane_base + 128 + c * 32, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+            tmem_st32(lane_base + 128 + c * 32, v);
+          }
+        }
+        const float mref = m_ref == -INFINITY ? 0.f : m_ref;
+        const uint64_t sc2 = f32x2(p.scale_log2, p.scale_log2), nm2 = f32x2(-mref, -mref);
+        uint64_t l2 = f32x2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 64; e += 2) {
+            const int a = c * 64 + e;
+            const float2 y = f32x2_split(fma_f32x2(
+                f32x2(__uint_as_float(sr[a >> 5][a & 31]), __uint_as_float(sr[a >> 5][(a + 1) & 31])), sc2, nm2));
+            const float p0 = exp2f(y.x), p1 = exp2f(y.y);
+            l2 = add_f32x2(l2, f32x2(p0, p1));
+            pk[e / 2] = Half16<T>::pack(p0, p1);
+          }
+          tmem_st32(lane_base + c * 32, pk);
+        }
+        const float2 ls = f32x2_split(l2);
+        l += ls.x + ls.y;
+        if (t == t_lo && clears) {
+          if (!wait(&v_full[vfirst % C::kV], vfirst / C::kV)) *abort_flag = 1;
+          uint4* row = reinterpret_cast<uint4*>(smem + C::oV + vfirst % C::kV * C::kTile + r * 128);
+#pragma unroll 1
+          for (int c = 0; c < D / 64 * 8; ++c) row[(c >> 3) * (kAtom / 16) + (c & 7)] = make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+        }
+        __syncwarp();
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[x]);
+      }
+      if (!ok) break;
+      if (t_hi <= t_lo) continue;
+      if (!mbar_wait_warp(&o_done[x], oc & 1, kBudgetNs, abort_flag, status)) {
+        fail(kErrTimeoutEpilogue);
+        break;
+      }
+      tc_fence_after();
+      const bool real = key.y > key.x;
+      const float inv = 1.f / l;
+      float odd = 0.f;  // becomes NaN when a value of the row is no number
+      T* orow = reinterpret_cast<T*>(p.o.p) + (int64_t)i * p.o.row + h * p.o.head;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t v[32];
+        tmem_ld32(lane_base + 128 + c * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float y = __uint_as_float(v[e]) * inv;
+          odd = fmaf(y, 0.f, odd);
+          v[e] = __float_as_uint(y);
+        }
+        if (real) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 o;
+            o.x = Half16<T>::pack(__uint_as_float(v[e + 0]), __uint_as_float(v[e + 1]));
+            o.y = Half16<T>::pack(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+            o.z = Half16<T>::pack(__uint_as_float(v[e + 4]), __uint_as_float(v[e + 5]));
+            o.w = Half16<T>::pack(__uint_as_float(v[e + 6]), __uint_as_float(v[e + 7]));
+            *reinterpret_cast<uint4*>(orow + c * 32 + e) = o;
+          }
+        }
+        __syncwarp();
+      }
+      if (real) p.lse[(int64_t)h * p.N + i] = (m_ref + log2f(l)) * kLn2;
+      // O is read: the next item's first product of this tile may overwrite it
+      tc_fence_before();
+      mbar_arrive(&o_empty[x]);
+      ++oc;
+      // rows that are no numbers although their scores are, and whose tiles hold foreign keys that were not cleared
+      bool again = real && odd != 0.f && l == l;
+      if (again) {
+        const int first = x == 0 || t_lo == t0 ? max(t_lo * BT, z) : t_lo * BT;
+        again = __ldg(p.start + i) > first || __ldg(p.end + i) < t_hi * BT;
+      }
+      uint32_t redo = __ballot_sync(0xffffffffu, again);
+      while (redo) {
+        const int b = __ffs((int)redo) - 1;
+        redo &= redo - 1;
+        fwd_row<T, D>(p, i - lane + b, h, lane);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
 }
 
 // ---------------------------------------------------------------------------------------- host side
@@ -274,6 +763,34 @@ PackedParams common_params(const char* what, const torch::Tensor& q, const torch
   return p;
 }
 
+// TMA maps of [rows, heads, D] tensors with boxes of box_rows rows of one head; bit i of the result: the i-th map's
+// coordinates are (d, row, head)
+template <size_t n>
+int tile_maps(const std::pair<const torch::Tensor*, CUtensorMap*> (&sides)[n], int box_rows) {
+  int swap = 0;
+  for (size_t i = 0; i < n; ++i) {
+    const torch::Tensor& t = *sides[i].first;
+    const Rows r = rows_of(t);
+    bool s = false;
+    *sides[i].second = tma_map_head_rows(
+        t.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r.p, t.size(2),
+        t.size(1), t.size(0), r.head, r.row, box_rows, &s);
+    swap |= (int)s << i;
+  }
+  return swap;
+}
+
+// a kernel's attributes belong to a device: each caller (each F) runs f once for each device that it is used on
+template <typename F>
+void once_per_device(int device, F&& f) {
+  static std::atomic<uint64_t> done{0};
+  TORCH_CHECK(device >= 0 && device < 64, "bad device index");
+  if (!(done.load(std::memory_order_acquire) >> device & 1)) {
+    f();
+    done.fetch_or(uint64_t(1) << device, std::memory_order_release);
+  }
+}
+
 template <typename F>
 void by_type(const torch::Tensor& q, F&& f) {
   const bool wide = q.size(2) == 128;
@@ -303,7 +820,19 @@ std::tuple<torch::Tensor, torch::Tensor> packed_attn_fwd(const torch::Tensor& q,
   c10::cuda::CUDAGuard g(q.device());
   auto st = at::cuda::getCurrentCUDAStream();
   by_type(q, [&](auto t, auto d) {
-    fwd_rows_kernel<decltype(t), d()><<<dim3((unsigned)((p.N + kRowWarps - 1) / kRowWarps), (unsigned)p.H), kRowWarps * 32, 0, st>>>(p);
+    constexpr int D = d();
+    using C = FwdCfg<D>;
+    FwdMaps maps;
+    const std::pair<const torch::Tensor*, CUtensorMap*> sides[] = {{&q, &maps.q}, {&k, &maps.k}, {&v, &maps.v}};
+    maps.swap = tile_maps(sides, BT);
+    once_per_device(q.device().index(), [] {
+      C10_CUDA_CHECK(cudaFuncSetAttribute(fwd_tc_kernel<decltype(t), D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          C::kSmem));
+    });
+    const int64_t tiles = (p.N + BT - 1) / BT;
+    const int64_t items = p.H / p.KV % 2 == 0 ? tiles * (p.H / 2) : (tiles + 1) / 2 * p.H;
+    TORCH_CHECK_VALUE(items < (int64_t(1) << 31), what, ": too many rows or heads");
+    fwd_tc_kernel<decltype(t), D><<<(unsigned)items, 320, C::kSmem, st>>>(maps, p, status_ptr(q.device().index()));
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {out, lse};

@@ -183,6 +183,33 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// ----------------------------------------------------------------------------------- work stealing
+// A running CTA takes over a block of its own grid that has not started: the request completes on `bar` with 16
+// bytes at `resp` (16-byte aligned), which say whether there was one and which. Nothing is shared between
+// launches, so grids of the same kernel may overlap. After a refusal no further request may follow.
+__device__ __forceinline__ void clc_request(void* resp, uint64_t* bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(resp)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// The x coordinate of the block taken over, or -1.
+__device__ __forceinline__ int clc_block(const void* resp) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t.reg .b32 y, z, w;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, r;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(resp))
+      : "memory");
+  return ok ? (int)x : -1;
+}
+
 // ----------------------------------------------------------------------------------- CTA pairs
 // A cluster of two CTAs running one 256-row tcgen05 MMA (cta_group::2). The even CTA (rank 0) is the
 // leader: it issues the MMAs, which read each CTA's half of the operands at the same shared-memory

@@ -27,4 +27,12 @@ struct Half16<__half> {
   }
 };
 
+// Instruction descriptor for kind::f16 with both operands of type T and f32 accumulation.
+template <typename T>
+__host__ __device__ constexpr uint32_t umma_idesc_16(int M, int N, bool a_mn, bool b_mn) {
+  return (1u << 4) | (Half16<T>::kFormat << 7) | (Half16<T>::kFormat << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+         (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+
 }  // namespace br

@@ -136,6 +136,35 @@ def test_nothing_crosses_a_border(cuda, D, what):
     assert (lse[:, sum(lengths):] == 7.0).all()
 
 
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("H,KV", [(4, 2), (3, 3)])
+def test_nothing_crosses_a_border_into_a_long_sequence(cuda, H, KV, window):
+    """One value in each input of a short sequence that is no number: every row tile of the long sequence behind it
+    starts in the tile that holds it, and the rows at the long one's end share a tile with the next."""
+    packed, check_status = _ops()
+    lengths, D = [60, 1500, 2, 700], 128
+    n = sum(lengths)
+    q, k, v = (t.clone() for t in _make(n, H, KV, D, torch.bfloat16, "plain"))
+    do = _make(n, H, KV, D, torch.bfloat16, "plain", 1)[0]
+    start, end = (t.cuda() for t in spans(lengths, n))
+    good = torch.ones(n, dtype=torch.bool, device="cuda")
+    good[:60] = False
+    good[1560:1562] = False
+    clean = attention(*(torch.where(good[:, None, None], t, torch.zeros_like(t)) for t in (q, k, v)), start, end, window,
+                      1 / math.sqrt(D), torch.where(good[:, None, None], do, torch.zeros_like(do)))
+    for t in (q, k, v, do):
+        t[59, :, 5] = math.inf
+        t[1561, 0, 100] = math.nan
+    out, lse = packed.attention_fwd(q, k, v, start, end, window=window)
+    grads = packed.attention_bwd(q, k, v, out, lse, do, start, end, window=window)
+    torch.cuda.synchronize()
+    assert check_status() == 0
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        value, tol = clean[name]
+        _within(got[good], (value[good], tol[good]), name)
+    _within(lse[:, good], tuple(t[:, good] for t in clean["lse"]), "lse")
+
+
 def test_bad_spans_stay_inside(cuda):
     """Spans that are none (negative, reversed, past the end): no fault and no error code, other rows untouched."""
     packed, check_status = _ops()
