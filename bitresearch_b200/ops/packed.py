@@ -11,8 +11,8 @@ padding rows hold; rows of no sequence are left as they were in every output (ze
 Spans must be those of sequences that follow one another; any other contents give wrong values but read and
 write no row outside the tensors.
 
-Calls run on the current stream of the tensors' device, in a captured graph too, allocate only the outputs and
-``delta`` when they are not given, and give the same bits for the same inputs. Wrong arguments raise ``ValueError``.
+Calls run on the current stream of the tensors' device, in a captured graph too, allocate only the outputs and the
+backward's scratch when they are not given, and give the same bits for the same inputs. Wrong arguments raise ``ValueError``.
 """
 from __future__ import annotations
 
@@ -51,13 +51,18 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start: torc
     return ext().packed_attn_fwd(q, k, v, start, end, window, scale, out, lse)
 
 
+def bwd_scratch(rows: int, heads: int) -> int:
+    """Entries of the fp32 scratch of :func:`attention_bwd`: two per head and row, rows rounded up to 128."""
+    return 2 * heads * ((rows + 127) // 128 * 128)
+
+
 def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
                   dout: torch.Tensor, start: torch.Tensor, end: torch.Tensor, window: int = 0,
                   scale: float | None = None, dq: torch.Tensor | None = None, dk: torch.Tensor | None = None,
                   dv: torch.Tensor | None = None,
-                  delta: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                  scratch: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(dq, dk, dv)`` of :func:`attention_fwd` for the gradient ``dout`` of ``out``, with the ``out`` and ``lse``
-    that it returned. Gradients of a kv head are summed over its query heads. ``delta`` is fp32 ``[H, N]`` of
-    scratch."""
+    that it returned. Gradients of a kv head are summed over its query heads. ``scratch`` is fp32 memory of
+    :func:`bwd_scratch` entries that no other call uses at the same time."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
-    return ext().packed_attn_bwd(q, k, v, out, lse, dout, start, end, window, scale, dq, dk, dv, delta)
+    return ext().packed_attn_bwd(q, k, v, out, lse, dout, start, end, window, scale, dq, dk, dv, scratch)

@@ -20,8 +20,10 @@
 // tiles' rows: a row that came out as no number and has such keys is computed alone, from its own keys
 // (fwd_row). That can be the case only within 256 rows of a border, so its cost stays bounded.
 //
-// Row by row (the backward, and the rows that a tile's product spoils): one warp per row and head, a lane holds
-// D / 32 of the row's values in fp32, a score is a warp-wide sum.
+// Backward: dQ, then dK/dV, on tcgen05 tiles of the same kind (described at the kernels).
+//
+// Row by row (the rows that a tile's product spoils): one warp per row and head, a lane holds D / 32 of the row's
+// values in fp32, a score is a warp-wide sum.
 #include <torch/extension.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -54,7 +56,8 @@ struct PackedParams {
   const int* start;
   const int* end;
   float* lse;    // [H, N], natural log
-  float* delta;  // [H, N]
+  float2* stat;  // backward scratch [H, Np]: (lse in log2 units, delta) of each row; (inf, 0) for rows of no sequence
+  int Np;        // N rounded up to whole tiles
 };
 
 // ---------------------------------------------------------------------------------------- row by row
@@ -142,7 +145,7 @@ __device__ __noinline__ void fwd_row(const PackedParams& p, int i, int h, int la
 }
 
 template <typename T, int D>
-__device__ __forceinline__ void dq_row(const PackedParams& p, int i, int h, int lane, float delta) {
+__device__ __noinline__ void dq_row(const PackedParams& p, int i, int h, int half, int lane, float2 stat) {
   constexpr int E = D / 32;
   const int2 key = keys_of(p, i);
   if (key.y <= key.x) return;
@@ -150,67 +153,53 @@ __device__ __forceinline__ void dq_row(const PackedParams& p, int i, int h, int 
   float q[E], d[E], acc[E] = {};
   load_row<T, D>(p.q, i, h, lane, q);
   load_row<T, D>(p.dout, i, h, lane, d);
-  const float lse2 = p.lse[(int64_t)h * p.N + i] * kLog2e;
-  for (int j = key.x; j < key.y; ++j) {
-    float k[E], v[E];
-    load_row<T, D>(p.k, j, g, lane, k);
-    load_row<T, D>(p.v, j, g, lane, v);
-    const float w = exp2f(dot(q, k) * p.scale_log2 - lse2);
-    const float ds = w * (dot(d, v) - delta);
+  for (int j0 = key.x; j0 < key.y; j0 += 4) {  // four keys at a time: their loads overlap
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(ds, k[e], acc[e]);
-  }
+    for (int u = 0; u < 4; ++u) {
+      float k[E], v[E];
+      const int j = min(j0 + u, key.y - 1);
+      load_row<T, D>(p.k, j, g, lane, k);
+      load_row<T, D>(p.v, j, g, lane, v);
+      const float w = exp2f(dot(q, k) * p.scale_log2 - stat.x);
+      const float ds = w * (dot(d, v) - stat.y);
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] *= p.scale;
-  store_row<T, D>(p.dq, i, h, lane, acc);
-}
-
-template <typename T, int D>
-__device__ __forceinline__ void dkv_row(const PackedParams& p, int j, int g, int lane) {
-  constexpr int E = D / 32;
-  const int hi = queries_of(p, j), group = p.H / p.KV;
-  if (hi <= j || __ldg(p.start + j) > j) return;
-  float k[E], v[E], dk[E] = {}, dv[E] = {};
-  load_row<T, D>(p.k, j, g, lane, k);
-  load_row<T, D>(p.v, j, g, lane, v);
-  for (int h = g * group; h < (g + 1) * group; ++h) {
-    for (int i = j; i < hi; ++i) {
-      float q[E], d[E];
-      load_row<T, D>(p.q, i, h, lane, q);
-      load_row<T, D>(p.dout, i, h, lane, d);
-      const int64_t at = (int64_t)h * p.N + i;
-      const float w = exp2f(dot(q, k) * p.scale_log2 - __ldg(p.lse + at) * kLog2e);
-      const float ds = w * (dot(d, v) - p.delta[at]);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        dv[e] = fmaf(w, d[e], dv[e]);
-        dk[e] = fmaf(ds, q[e], dk[e]);
-      }
+      for (int e = 0; e < E; ++e) acc[e] = j0 + u < key.y ? fmaf(ds, k[e], acc[e]) : acc[e];
     }
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) dk[e] *= p.scale;
-  store_row<T, D>(p.dk, j, g, lane, dk);
-  store_row<T, D>(p.dv, j, g, lane, dv);
+  for (int e = 0; e < E; ++e) acc[e] *= p.scale;
+  if (lane / 16 == half) store_row<T, D>(p.dq, i, h, lane, acc);  // the other half of the row is the other warp's
 }
 
-constexpr int kRowWarps = 8;
-
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32) dq_rows_kernel(PackedParams p) {
-  const int i = blockIdx.x * kRowWarps + (threadIdx.x >> 5), h = blockIdx.y, lane = threadIdx.x & 31;
-  if (i >= p.N) return;
-  float o[D / 32], d[D / 32];
-  load_row<T, D>(p.o, i, h, lane, o);
-  load_row<T, D>(p.dout, i, h, lane, d);
-  const float delta = dot(o, d);
-  if (lane == 0) p.delta[(int64_t)h * p.N + i] = delta;
-  dq_row<T, D>(p, i, h, lane, delta);
-}
-template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32) dkv_rows_kernel(PackedParams p) {
-  const int j = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  if (j < p.N) dkv_row<T, D>(p, j, blockIdx.y, threadIdx.x & 31);
+__device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool want_dk, int lane) {
+  constexpr int E = D / 32;
+  const int hi = queries_of(p, j), group = p.H / p.KV;
+  float k[E], v[E], acc[E] = {};
+  load_row<T, D>(p.k, j, g, lane, k);
+  load_row<T, D>(p.v, j, g, lane, v);
+  for (int h = g * group; h < (g + 1) * group; ++h) {
+    const float2* stat = p.stat + (int64_t)h * p.Np;
+    for (int i0 = j; i0 < hi; i0 += 4) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float q[E], d[E];
+        const int i = min(i0 + u, hi - 1);
+        load_row<T, D>(p.q, i, h, lane, q);
+        load_row<T, D>(p.dout, i, h, lane, d);
+        const float2 st = stat[i];
+        const float w = exp2f(dot(q, k) * p.scale_log2 - st.x);
+        const float ds = w * (dot(d, v) - st.y);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = i0 + u < hi ? fmaf(want_dk ? ds : w, want_dk ? q[e] : d[e], acc[e]) : acc[e];
+      }
+    }
+  }
+  if (want_dk) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= p.scale;
+  }
+  store_row<T, D>(want_dk ? p.dk : p.dv, j, g, lane, acc);
 }
 
 // ---------------------------------------------------------------------------------------- forward, tcgen05
@@ -685,6 +674,552 @@ __global__ void __launch_bounds__(320, 1) fwd_tc_kernel(const __grid_constant__ 
   }
 }
 
+// ---------------------------------------------------------------------------------------- backward, tcgen05
+// Two kernels, so that no sum is shared between blocks and the results do not depend on the schedule: dQ (one block
+// per 128 query rows and head) and dK/dV (one block per 128 key rows and kv head). Both recompute the scores,
+// 64 keys or queries at a time, 320 threads: warp 0 loads (TMA), warp 1 issues the MMAs, warps 2-9 turn scores
+// into P and dS, one tile row per thread, warps w and w + 4 sharing the rows of TMEM lane group w % 4 and
+// splitting the block's 64 columns. P and dS are rounded to 16 bits for their products (half a step, relative to
+// each entry); everything else is fp32. A warp writes its 16-bit results over the scores that it has itself read.
+constexpr int BB = 64;  // keys (dQ) or queries (dK/dV) of a block
+constexpr int kAtom64 = BB * 128;
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// 32 fp32 columns of a TMEM row, times f, to 32 16-bit values in memory; true if one of them is no number
+template <typename T>
+__device__ __forceinline__ bool store_cols(uint32_t taddr, float f, T* dst, bool write) {
+  uint32_t v[32];
+  tmem_ld32(taddr, v);
+  tmem_ld_wait();
+  float odd = 0.f;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) {
+    const float y = __uint_as_float(v[e]) * f;
+    odd = fmaf(y, 0.f, odd);
+    v[e] = __float_as_uint(y);
+  }
+  if (write) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+      uint4 o;
+      o.x = Half16<T>::pack(__uint_as_float(v[e + 0]), __uint_as_float(v[e + 1]));
+      o.y = Half16<T>::pack(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+      o.z = Half16<T>::pack(__uint_as_float(v[e + 4]), __uint_as_float(v[e + 5]));
+      o.w = Half16<T>::pack(__uint_as_float(v[e + 6]), __uint_as_float(v[e + 7]));
+      *reinterpret_cast<uint4*>(dst + e) = o;
+    }
+  }
+  __syncwarp();
+  return odd != 0.f;
+}
+
+// dQ. TMEM: two score sets (set s: S at [128s, +64), dP at [128s + 64, +64)), so that block j + 1's scores are
+// computed while block j is turned into dS; dQ at [256, +D); the block's Q and dO rows as 16-bit pairs at [384, +D/2)
+// and [448, +D/2): the S and dP products read only K and V from shared memory. The kernel also computes
+// delta = rowsum(dO o O) and leaves (lse, delta) of each row for the dK/dV kernel.
+template <int D>
+struct DqCfg {
+  static constexpr int kTile = BB * D * 2;
+  static constexpr int kStages = 6;
+  static constexpr int oK = 0, oV = kStages * kTile, oSum = oV + kStages * kTile;  // oSum: [2][128] half-row sums
+  static constexpr int oBar = oSum + 1024;
+  static constexpr int kSmem = oBar + 256 + 1024;
+  static_assert(kSmem <= 232448, "dQ shared memory");
+};
+
+struct DqMaps {
+  CUtensorMap k, v;
+  int swap;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(320, 1) dq_tc_kernel(const __grid_constant__ DqMaps maps,
+                                                       const __grid_constant__ PackedParams p, int* status) {
+  using C = DqCfg<D>;
+  constexpr int kAtoms = D / 64;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
+  uint64_t* q_full = bars + 0;
+  uint64_t* done = bars + 1;
+  uint64_t* s_full = bars + 2;  // [2]
+  uint64_t* p_full = bars + 4;  // [2], by block parity: a warp group one block ahead arrives on the other barrier
+  uint64_t* kv_full = bars + 6;
+  uint64_t* kv_empty = kv_full + C::kStages;
+  static_assert(6 + 2 * C::kStages <= 28, "barrier region");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int tile = (int)gridDim.x / p.H - 1 - (int)blockIdx.x / p.H, h = blockIdx.x % p.H;  // late rows first
+  const int kvh = h / (p.H / p.KV), q0 = tile * BT;
+  const int warp = warp_id();
+  if (device_failed(status)) return;
+  // spans never decrease along the rows: the first row has the first key
+  const int kb_hi = min(q0 + BT, p.N) - 1 >> 6;
+  const int kb_lo = min(max(keys_of(p, q0).x, 0) >> 6, kb_hi);
+  const int nb = kb_hi - kb_lo + 1;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 256);  // every softmax thread has stored its Q or dO row in TMEM
+    mbar_init(done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 256);
+    }
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto fail = [&](int code) {
+    *abort_flag = 1;
+    if (status) atomicCAS(status, 0, code);
+  };
+  auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, kBudgetNs, abort_flag, status); };
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int j = 0;
+      bool ok = true;
+      for (; j < nb; ++j) {
+        const int st = j % C::kStages;
+        if (!wait(&kv_empty[st], (j / C::kStages) ^ 1)) {
+          ok = false;
+          break;
+        }
+        const int k0 = (kb_lo + j) * BB;
+        mbar_arrive_expect_tx(&kv_full[st], 2 * C::kTile);
+        load_tile(&maps.k, maps.swap & 1, &kv_full[st], smem + C::oK + st * C::kTile, kvh, k0, kAtoms, kAtom64);
+        load_tile(&maps.v, maps.swap & 2, &kv_full[st], smem + C::oV + st * C::kTile, kvh, k0, kAtoms, kAtom64);
+      }
+      if (!ok) {
+        fail(kErrTimeoutProducer);
+        for (int g = max(0, j - C::kStages); g < j; ++g)
+          mbar_wait(&kv_full[g % C::kStages], (g / C::kStages) & 1, kDrainNs, nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = umma_idesc_16<T>(BT, BB, false, false);
+      constexpr uint32_t idesc_q = umma_idesc_16<T>(BT, D, false, true);
+      bool ok = wait(q_full, 0);
+      auto issue_s = [&](int j) -> bool {
+        const int st = j % C::kStages, set = j & 1;
+        if (!wait(&kv_full[st], j / C::kStages)) return false;
+        tc_fence_after();
+        const uint32_t k_addr = smem_u32(smem + C::oK + st * C::kTile), v_addr = smem_u32(smem + C::oV + st * C::kTile);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kAtom64 + (kk & 3) * 32;
+          umma_bf16_ts(tmem + set * 128, tmem + 384 + kk * 8, umma_desc_sw128(k_addr + off, 16, 1024), idesc_s,
+                       kk > 0 ? 1u : 0u);
+          umma_bf16_ts(tmem + set * 128 + 64, tmem + 448 + kk * 8, umma_desc_sw128(v_addr + off, 16, 1024), idesc_s,
+                       kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[set]);
+        return true;
+      };
+      if (ok) ok = issue_s(0);
+      for (int j = 0; j < nb && ok; ++j) {
+        if (j + 1 < nb && !issue_s(j + 1)) ok = false;
+        if (!ok || !wait(&p_full[j & 1], j >> 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int st = j % C::kStages;
+        const uint32_t k_addr = smem_u32(smem + C::oK + st * C::kTile);
+        // dS of keys 32h .. 32h + 31 sits at columns 128 set + 32h .. + 15
+#pragma unroll
+        for (int kk = 0; kk < BB / 16; ++kk)
+          umma_bf16_ts(tmem + 256, tmem + (j & 1) * 128 + (kk >> 1) * 32 + (kk & 1) * 8,
+                       umma_desc_sw128(k_addr + kk * 2048, kAtom64, 1024), idesc_q, (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&kv_empty[st]);
+      }
+      if (!ok) fail(kErrTimeoutMma);
+      umma_commit(done);
+      mbar_wait(done, 0, kBudgetNs, nullptr);
+    }
+  } else {
+    const int wq = warp & 3, lane = lane_id(), half = (warp - 2) >> 2;
+    const int r = wq * 32 + lane, i = q0 + r, ic = min(i, p.N - 1);
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+    const int2 key = i < p.N ? keys_of(p, i) : make_int2(0, 0);
+    const bool real = key.y > key.x;
+    {
+      // this row's Q (first warp of the row) or dO (second warp) into TMEM: the A operands of S and dP
+      const Rows& src = half == 0 ? p.q : p.dout;
+      const uint4* g = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(src.p) + ic * src.row + h * src.head);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint4 a = __ldg(g + c * 8 + e);
+          w[4 * e] = a.x;
+          w[4 * e + 1] = a.y;
+          w[4 * e + 2] = a.z;
+          w[4 * e + 3] = a.w;
+        }
+        tmem_st32(lane_base + 384 + 64 * half + 32 * c, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(q_full);
+    }
+    // delta: the two warps of a row each reduce half of its values and meet in shared memory
+    float2 stat;
+    {
+      float* sums = reinterpret_cast<float*>(smem + C::oSum);
+      const uint4* og = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.o.p) + ic * p.o.row + h * p.o.head +
+                                                       half * (D / 2));
+      const uint4* dg = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.dout.p) + ic * p.dout.row +
+                                                       h * p.dout.head + half * (D / 2));
+      float acc = 0.f;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) {
+        const uint4 a = __ldg(og + e), b = __ldg(dg + e);
+        const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 u = Half16<T>::unpack(x[k]), w = Half16<T>::unpack(y[k]);
+          acc = fmaf(u.x, w.x, fmaf(u.y, w.y, acc));
+        }
+      }
+      sums[half * 128 + r] = acc;
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps
+      stat = real ? make_float2(p.lse[(int64_t)h * p.N + i] * kLog2e, sums[r] + sums[128 + r])
+                  : make_float2(INFINITY, 0.f);
+      if (half == 0) p.stat[(int64_t)h * p.Np + i] = stat;
+    }
+    const int z = __ldg(p.start + q0);  // keys before it are foreign to every row of the tile: all in block kb_lo
+    bool ok = true;
+    for (int j = 0; j < nb; ++j) {
+      const int set = j & 1;
+      if (!mbar_wait_warp(&s_full[set], (j >> 1) & 1, kBudgetNs, abort_flag, status)) {
+        fail(kErrTimeoutEpilogue);
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int k0 = (kb_lo + j) * BB + half * 32;
+      uint32_t sv[32], dv[32], pk[16];
+      tmem_ld32(lane_base + set * 128 + half * 32, sv);
+      tmem_ld32(lane_base + set * 128 + 64 + half * 32, dv);
+      tmem_ld_wait();
+      // dS = P (dP - delta), 0 where the row does not see the key
+      auto body = [&](auto masked) {
+        constexpr bool kMasked = decltype(masked)::value;
+        uint32_t vis = 0xffffffffu;
+        if constexpr (kMasked) vis = range_mask32(key.x - k0, key.y - k0);
+        const uint64_t dl2 = f32x2(stat.y, stat.y);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float p0 = exp2f(fmaf(__uint_as_float(sv[e]), p.scale_log2, -stat.x));
+          const float p1 = exp2f(fmaf(__uint_as_float(sv[e + 1]), p.scale_log2, -stat.x));
+          float2 g = f32x2_split(
+              mul_f32x2(f32x2(p0, p1), sub_f32x2(f32x2(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), dl2)));
+          if constexpr (kMasked) {
+            g.x = ((vis >> e) & 1u) ? g.x : 0.f;
+            g.y = ((vis >> (e + 1)) & 1u) ? g.y : 0.f;
+          }
+          pk[e / 2] = Half16<T>::pack(g.x, g.y);
+        }
+      };
+      if (__all_sync(0xffffffffu, key.x <= k0 && key.y >= k0 + 32)) {
+        body(std::false_type{});
+      } else {
+        body(std::true_type{});
+      }
+      if (j == 0 && half == 0 && r < BB && kb_lo * BB + r < z) {
+        uint4* row = reinterpret_cast<uint4*>(smem + C::oK + r * 128);
+#pragma unroll 1
+        for (int c = 0; c < D / 64 * 8; ++c) row[(c >> 3) * (kAtom64 / 16) + (c & 7)] = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+      }
+      __syncwarp();
+      tmem_st16(lane_base + set * 128 + half * 32, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[j & 1]);
+    }
+    if (ok && mbar_wait_warp(done, 0, kBudgetNs, abort_flag, status)) {
+      tc_fence_after();
+      T* row = reinterpret_cast<T*>(p.dq.p) + (int64_t)i * p.dq.row + h * p.dq.head;
+      bool odd = false;
+#pragma unroll 1
+      for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c)
+        odd |= store_cols<T>(lane_base + 256 + c * 32, p.scale, row + c * 32, real);
+      // as in the forward: no number, though the scores are, and foreign keys among the tile's that were not cleared
+      bool again = real && odd && stat.x == stat.x;
+      if (again) again = __ldg(p.start + i) > max(kb_lo * BB, z) || __ldg(p.end + i) < (kb_hi + 1) * BB;
+      uint32_t redo = __ballot_sync(0xffffffffu, again);
+      while (redo) {
+        const int b = __ffs((int)redo) - 1;
+        redo &= redo - 1;
+        const float2 st = make_float2(__shfl_sync(0xffffffffu, stat.x, b), __shfl_sync(0xffffffffu, stat.y, b));
+        dq_row<T, D>(p, i - lane + b, h, half, lane, st);
+      }
+    } else if (ok) {
+      fail(kErrTimeoutEpilogue);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// dK and dV. TMEM: two score sets (set s: S^T at [128s, +64), dP^T at [128s + 64, +64)), dV at [256, +D), dK at
+// [384, +D). K and V stay in shared memory as the A operands of S^T and dP^T; blocks of 64 queries (Q, dO, their
+// lse and delta) go through a ring, head after head of the kv head's group.
+template <int D>
+struct DkvCfg {
+  static constexpr int kTile = BT * D * 2, kBlock = BB * D * 2;
+  static constexpr int kStages = 4;
+  static constexpr int oK = 0, oV = kTile, oQ = 2 * kTile, oD = oQ + kStages * kBlock, oStat = oD + kStages * kBlock;
+  static constexpr int oBar = oStat + kStages * BB * 8;
+  static constexpr int kSmem = oBar + 256 + 1024;
+  static_assert(kSmem <= 232448, "dK/dV shared memory");
+};
+
+struct DkvMaps {
+  CUtensorMap k, v, q, d;
+  int swap_kv, swap_qd;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(320, 1) dkv_tc_kernel(const __grid_constant__ DkvMaps maps,
+                                                        const __grid_constant__ PackedParams p, int* status) {
+  using C = DkvCfg<D>;
+  constexpr int kAtoms = D / 64;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
+  uint64_t* kv_full = bars + 0;
+  uint64_t* done = bars + 1;
+  uint64_t* s_full = bars + 2;  // [2]
+  uint64_t* p_full = bars + 4;  // [2], by iteration parity
+  uint64_t* qd_full = bars + 6;
+  uint64_t* qd_empty = qd_full + C::kStages;
+  static_assert(6 + 2 * C::kStages <= 28, "barrier region");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float2* stat = reinterpret_cast<float2*>(smem + C::oStat);
+
+  const int kvh = blockIdx.x % p.KV, k0 = (int)blockIdx.x / p.KV * BT, group = p.H / p.KV;
+  const int warp = warp_id();
+  if (device_failed(status)) return;
+  // spans never decrease along the rows: the last row is seen by the last query
+  const int k_last = min(k0 + BT, p.N) - 1;
+  const int qb_lo = k0 / BB, qb_hi = (max(queries_of(p, k_last), k_last + 1) - 1) / BB;
+  const int nq = qb_hi - qb_lo + 1, iters = nq * group;
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    mbar_init(done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 256);
+    }
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&qd_full[i], 1);
+      mbar_init(&qd_empty[i], 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto fail = [&](int code) {
+    *abort_flag = 1;
+    if (status) atomicCAS(status, 0, code);
+  };
+  auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, kBudgetNs, abort_flag, status); };
+
+  if (warp == 0) {
+    if (elect_one()) {
+      mbar_arrive_expect_tx(kv_full, 2 * C::kTile);
+      load_tile(&maps.k, maps.swap_kv & 1, kv_full, smem + C::oK, kvh, k0, kAtoms, kAtom);
+      load_tile(&maps.v, maps.swap_kv & 2, kv_full, smem + C::oV, kvh, k0, kAtoms, kAtom);
+      int it = 0;
+      bool ok = true;
+      for (; it < iters; ++it) {
+        const int st = it % C::kStages;
+        if (!wait(&qd_empty[st], (it / C::kStages) ^ 1)) {
+          ok = false;
+          break;
+        }
+        const int h = kvh * group + it / nq, q0 = (qb_lo + it % nq) * BB;
+        mbar_arrive_expect_tx(&qd_full[st], 2 * C::kBlock + BB * 8);
+        load_tile(&maps.q, maps.swap_qd & 1, &qd_full[st], smem + C::oQ + st * C::kBlock, h, q0, kAtoms, kAtom64);
+        load_tile(&maps.d, maps.swap_qd & 2, &qd_full[st], smem + C::oD + st * C::kBlock, h, q0, kAtoms, kAtom64);
+        bulk_load(stat + st * BB, p.stat + (int64_t)h * p.Np + q0, BB * 8, &qd_full[st]);
+      }
+      if (!ok) {
+        fail(kErrTimeoutProducer);
+        mbar_wait(kv_full, 0, kDrainNs, nullptr);
+        for (int g = max(0, it - C::kStages); g < it; ++g)
+          mbar_wait(&qd_full[g % C::kStages], (g / C::kStages) & 1, kDrainNs, nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = umma_idesc_16<T>(BT, BB, false, false);
+      constexpr uint32_t idesc_g = umma_idesc_16<T>(BT, D, false, true);
+      const uint32_t k_addr = smem_u32(smem + C::oK), v_addr = smem_u32(smem + C::oV);
+      bool ok = wait(kv_full, 0);
+      auto issue_s = [&](int it) -> bool {
+        const int st = it % C::kStages, set = it & 1;
+        if (!wait(&qd_full[st], it / C::kStages)) return false;
+        tc_fence_after();
+        const uint32_t q_addr = smem_u32(smem + C::oQ + st * C::kBlock), d_addr = smem_u32(smem + C::oD + st * C::kBlock);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t offa = (kk >> 2) * kAtom + (kk & 3) * 32, offb = (kk >> 2) * kAtom64 + (kk & 3) * 32;
+          umma_bf16_ss(tmem + set * 128, umma_desc_sw128(k_addr + offa, 16, 1024),
+                       umma_desc_sw128(q_addr + offb, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+          umma_bf16_ss(tmem + set * 128 + 64, umma_desc_sw128(v_addr + offa, 16, 1024),
+                       umma_desc_sw128(d_addr + offb, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[set]);
+        return true;
+      };
+      if (ok) ok = issue_s(0);
+      for (int it = 0; it < iters && ok; ++it) {
+        if (it + 1 < iters && !issue_s(it + 1)) ok = false;
+        if (!ok || !wait(&p_full[it & 1], it >> 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int st = it % C::kStages, set = it & 1;
+        const uint32_t q_addr = smem_u32(smem + C::oQ + st * C::kBlock), d_addr = smem_u32(smem + C::oD + st * C::kBlock);
+        // P^T and dS^T of queries 32h .. 32h + 31 sit at columns 32h .. + 15 of S^T and dP^T
+#pragma unroll
+        for (int kk = 0; kk < BB / 16; ++kk) {
+          const uint32_t acc = (it > 0 || kk > 0) ? 1u : 0u;
+          const uint32_t col = tmem + set * 128 + (kk >> 1) * 32 + (kk & 1) * 8;
+          umma_bf16_ts(tmem + 256, col, umma_desc_sw128(d_addr + kk * 2048, kAtom64, 1024), idesc_g, acc);
+          umma_bf16_ts(tmem + 384, col + 64, umma_desc_sw128(q_addr + kk * 2048, kAtom64, 1024), idesc_g, acc);
+        }
+        umma_commit(&qd_empty[st]);
+      }
+      if (!ok) fail(kErrTimeoutMma);
+      umma_commit(done);
+      mbar_wait(done, 0, kBudgetNs, nullptr);
+    }
+  } else {
+    const int wq = warp & 3, lane = lane_id(), half = (warp - 2) >> 2;
+    const int r = wq * 32 + lane, j = k0 + r;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+    // the queries that see this key row (none for a row of no sequence)
+    const bool real = j < p.N && __ldg(p.start + j) <= j && queries_of(p, j) > j;
+    const int q_hi = real ? queries_of(p, j) : 0;
+    const int z = __ldg(p.end + k_last);  // queries from here on are foreign to every key of the tile: all in block qb_hi
+    bool ok = true;
+    for (int it = 0; it < iters; ++it) {
+      const int set = it & 1, st = it % C::kStages;
+      if (!mbar_wait_warp(&s_full[set], (it >> 1) & 1, kBudgetNs, abort_flag, status)) {
+        fail(kErrTimeoutEpilogue);
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int q0 = (qb_lo + it % nq) * BB + half * 32;
+      const float4* ls = reinterpret_cast<const float4*>(stat + st * BB + half * 32);
+      uint32_t sv[32], dv[32], pp[16], ss[16];
+      tmem_ld32(lane_base + set * 128 + half * 32, sv);
+      tmem_ld32(lane_base + set * 128 + 64 + half * 32, dv);
+      tmem_ld_wait();
+      auto body = [&](auto masked) {
+        constexpr bool kMasked = decltype(masked)::value;
+        uint32_t vis = 0xffffffffu;
+        if constexpr (kMasked) vis = range_mask32(real ? j - q0 : 32, q_hi - q0);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float4 a = ls[e / 2];  // (lse, delta) of two queries
+          float p0 = exp2f(fmaf(__uint_as_float(sv[e]), p.scale_log2, -a.x));
+          float p1 = exp2f(fmaf(__uint_as_float(sv[e + 1]), p.scale_log2, -a.z));
+          float2 g = f32x2_split(mul_f32x2(
+              f32x2(p0, p1), sub_f32x2(f32x2(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), f32x2(a.y, a.w))));
+          if constexpr (kMasked) {
+            const bool v0 = (vis >> e) & 1u, v1 = (vis >> (e + 1)) & 1u;
+            p0 = v0 ? p0 : 0.f;
+            p1 = v1 ? p1 : 0.f;
+            g.x = v0 ? g.x : 0.f;
+            g.y = v1 ? g.y : 0.f;
+          }
+          pp[e / 2] = Half16<T>::pack(p0, p1);
+          ss[e / 2] = Half16<T>::pack(g.x, g.y);
+        }
+      };
+      if (__all_sync(0xffffffffu, real && j <= q0 && q_hi >= q0 + 32)) {
+        body(std::false_type{});
+      } else {
+        body(std::true_type{});
+      }
+      if (it % nq == nq - 1 && half == 0 && r < BB && qb_hi * BB + r >= z) {
+        uint4* row = reinterpret_cast<uint4*>(smem + C::oQ + st * C::kBlock + r * 128);
+        uint4* dow = reinterpret_cast<uint4*>(smem + C::oD + st * C::kBlock + r * 128);
+#pragma unroll 1
+        for (int c = 0; c < D / 64 * 8; ++c)
+          row[(c >> 3) * (kAtom64 / 16) + (c & 7)] = dow[(c >> 3) * (kAtom64 / 16) + (c & 7)] = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+      }
+      __syncwarp();
+      tmem_st16(lane_base + set * 128 + half * 32, pp);
+      tmem_st16(lane_base + set * 128 + 64 + half * 32, ss);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[it & 1]);
+    }
+    if (ok && mbar_wait_warp(done, 0, kBudgetNs, abort_flag, status)) {
+      tc_fence_after();
+      // half 0 writes dV, half 1 writes dK
+      const Rows& to = half ? p.dk : p.dv;
+      T* row = reinterpret_cast<T*>(to.p) + (int64_t)j * to.row + kvh * to.head;
+      bool odd = false;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c)
+        odd |= store_cols<T>(lane_base + (half ? 384 : 256) + c * 32, half ? p.scale : 1.f, row + c * 32, real);
+      // no number, and foreign queries among the tile's that were not cleared
+      bool again = real && odd;
+      if (again) again = __ldg(p.start + j) > k0 || __ldg(p.end + j) < min(z, (qb_hi + 1) * BB);
+      uint32_t redo = __ballot_sync(0xffffffffu, again);
+      while (redo) {
+        const int b = __ffs((int)redo) - 1;
+        redo &= redo - 1;
+        dkv_row<T, D>(p, j - lane + b, kvh, half, lane);
+      }
+    } else if (ok) {
+      fail(kErrTimeoutEpilogue);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 // ---------------------------------------------------------------------------------------- host side
 void check_rows(const torch::Tensor& t, const char* what, const char* name, int64_t N, int64_t heads, int64_t D,
                 const torch::Tensor& like) {
@@ -842,16 +1377,26 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
     const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& out,
     const torch::Tensor& lse, const torch::Tensor& dout, const torch::Tensor& start, const torch::Tensor& end,
     int64_t window, double scale, c10::optional<torch::Tensor> dq_, c10::optional<torch::Tensor> dk_,
-    c10::optional<torch::Tensor> dv_, c10::optional<torch::Tensor> delta_) {
+    c10::optional<torch::Tensor> dv_, c10::optional<torch::Tensor> scratch_) {
   const char* what = "packed attention_bwd";
   PackedParams p = common_params(what, q, k, v, start, end, window, scale);
-  const int64_t N = p.N, H = p.H, KV = p.KV, D = q.size(2);
-  check_rows(out, what, "out", N, H, D, q);
-  check_rows(dout, what, "dout", N, H, D, q);
+  const int64_t N = p.N, H = p.H, KV = p.KV;
+  check_rows(out, what, "out", N, H, q.size(2), q);
+  check_rows(dout, what, "dout", N, H, q.size(2), q);
   stat_rows(lse, what, "lse", H, q, false);
   torch::Tensor dq = out_rows(dq_, what, "dq", H, q), dk = out_rows(dk_, what, "dk", KV, q),
                 dv = out_rows(dv_, what, "dv", KV, q);
-  torch::Tensor delta = stat_rows(delta_, what, "delta", H, q, false);
+  p.Np = (int)((N + BT - 1) / BT * BT);
+  torch::Tensor scratch;
+  if (scratch_.has_value() && scratch_->defined()) {
+    scratch = *scratch_;
+    TORCH_CHECK_VALUE(scratch.scalar_type() == at::kFloat && scratch.is_contiguous() && scratch.numel() >= 2 * H * p.Np &&
+                          reinterpret_cast<uintptr_t>(scratch.data_ptr()) % 16 == 0,
+                      what, ": scratch must be contiguous float32 of ", std::to_string(2 * H * p.Np), " entries, 16-byte aligned");
+    TORCH_CHECK_VALUE(scratch.device() == q.device(), what, ": scratch is on another device than q");
+  } else {
+    scratch = torch::empty({2 * H * p.Np}, q.options().dtype(at::kFloat));
+  }
   for (const torch::Tensor* r : {&dq, &dk, &dv})
     for (const torch::Tensor* t : {&q, &k, &v, &out, &dout}) at::assert_no_overlap(*r, *t);
   TORCH_CHECK_VALUE(q.is_cuda(), what, ": q must be on a CUDA device");
@@ -862,14 +1407,29 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
   p.dk = rows_of(dk);
   p.dv = rows_of(dv);
   p.lse = lse.data_ptr<float>();
-  p.delta = delta.data_ptr<float>();
+  p.stat = reinterpret_cast<float2*>(scratch.data_ptr<float>());
   c10::cuda::CUDAGuard g(q.device());
   auto st = at::cuda::getCurrentCUDAStream();
   by_type(q, [&](auto t, auto d) {
-    const unsigned x = (unsigned)((N + kRowWarps - 1) / kRowWarps);
-    dq_rows_kernel<decltype(t), d()><<<dim3(x, (unsigned)H), kRowWarps * 32, 0, st>>>(p);
+    using T = decltype(t);
+    constexpr int D = d();
+    DqMaps a;
+    const std::pair<const torch::Tensor*, CUtensorMap*> kv64[] = {{&k, &a.k}, {&v, &a.v}};
+    a.swap = tile_maps(kv64, BB);
+    DkvMaps b;
+    const std::pair<const torch::Tensor*, CUtensorMap*> kv[] = {{&k, &b.k}, {&v, &b.v}}, qd[] = {{&q, &b.q}, {&dout, &b.d}};
+    b.swap_kv = tile_maps(kv, BT);
+    b.swap_qd = tile_maps(qd, BB);
+    once_per_device(q.device().index(), [] {
+      C10_CUDA_CHECK(cudaFuncSetAttribute(dq_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DqCfg<D>::kSmem));
+      C10_CUDA_CHECK(cudaFuncSetAttribute(dkv_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DkvCfg<D>::kSmem));
+    });
+    const int64_t tiles = p.Np / BT;
+    TORCH_CHECK_VALUE(tiles * H < (int64_t(1) << 31), what, ": too many rows or heads");
+    int* status = status_ptr(q.device().index());
+    dq_tc_kernel<T, D><<<(unsigned)(tiles * H), 320, DqCfg<D>::kSmem, st>>>(a, p, status);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
-    dkv_rows_kernel<decltype(t), d()><<<dim3(x, (unsigned)KV), kRowWarps * 32, 0, st>>>(p);
+    dkv_tc_kernel<T, D><<<(unsigned)(tiles * KV), 320, DkvCfg<D>::kSmem, st>>>(b, p, status);
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {dq, dk, dv};

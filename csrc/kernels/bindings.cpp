@@ -125,7 +125,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
     const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& out,
     const torch::Tensor& lse, const torch::Tensor& dout, const torch::Tensor& start, const torch::Tensor& end,
     int64_t window, double scale, c10::optional<torch::Tensor> dq, c10::optional<torch::Tensor> dk,
-    c10::optional<torch::Tensor> dv, c10::optional<torch::Tensor> delta);
+    c10::optional<torch::Tensor> dv, c10::optional<torch::Tensor> scratch);
 std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> distill_topk(
     const torch::Tensor& logits, const torch::Tensor& ids, const torch::Tensor& teacher,
     c10::optional<torch::Tensor> targets, double cap, double temperature, double alpha, double scale, bool need_grad,

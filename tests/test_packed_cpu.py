@@ -92,7 +92,8 @@ def test_attention_fwd_refuses(change, message):
     (lambda a: a.update(out=a["out"][:, :2]), "out must be"),
     (lambda a: a.update(lse=a["lse"].double()), "lse must be"),
     (lambda a: a.update(dq=a["k"].clone()), "dq must be"),
-    (lambda a: a.update(delta=torch.zeros(3, 8)), "delta must be"),
+    (lambda a: a.update(scratch=torch.zeros(2 * 4 * 128 - 1)), "scratch must be"),
+    (lambda a: a.update(scratch=torch.zeros(packed.bwd_scratch(8, 4)).half()), "scratch must be"),
     (lambda a: None, "CUDA device"),
 ])
 def test_attention_bwd_refuses(change, message):
