@@ -144,7 +144,11 @@ def test_strides_alignment_and_place(cuda, V, dt):
     M, K = 6, 12
     z, ids, u, y = _inputs(M, V, K, dt, 15.0, seed=3)
     args = dict(cap=15.0, temperature=2.0, alpha=0.5, scale=0.5)
-    _, rows, want = op(z, ids, u, y, **args)
+    # another alignment cuts the row into other vectors and adds its sums in another order, so the bits may differ: each
+    # call is held to the 64-bit form
+    r, g, rt, gt = (x.cuda() for x in reference(z, ids, u, y, 15.0, 2.0, 0.5, 0.5))
+    near = lambda rows, grad: bool(((rows.double() - r).abs() <= rt).all() and ((grad.double() - g).abs() <= gt).all())  # noqa: E731
+    _, rows, _ = op(z, ids, u, y, **args)
     for off, pad in ((0, 5), (1, 0), (3, 8)):
         wide = torch.full((M, V + off + pad), 9.0, device="cuda").to(dt)
         wide[:, off:off + V] = z
@@ -152,10 +156,10 @@ def test_strides_alignment_and_place(cuda, V, dt):
         wide_ids[:, 1:K + 1] = ids
         out = torch.full((M, V + 2), 9.0, device="cuda").to(dt)
         _, r1, _ = op(wide[:, off:off + V], wide_ids[:, 1:K + 1], u, y, grad=out[:, 1:V + 1], **args)
-        assert torch.equal(r1, rows) and torch.equal(out[:, 1:V + 1], want)
+        assert near(r1, out[:, 1:V + 1])
         assert (out[:, 0] == 9).all() and (out[:, -1] == 9).all()
         _, r2, g2 = op(wide[:, off:off + V], ids, u, y, grad=wide[:, off:off + V], **args)
-        assert torch.equal(r2, rows) and torch.equal(wide[:, off:off + V], want)
+        assert near(r2, wide[:, off:off + V])
         assert (wide[:, :off] == 9).all() and (wide[:, off + V:] == 9).all()
     l3, r3, none = op(z, ids, u, y, need_grad=False, **args)
     assert none is None and torch.equal(r3, rows)
