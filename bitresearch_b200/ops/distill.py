@@ -14,7 +14,8 @@ def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     ``loss = scale * sum(rows)`` (``scale`` defaults to ``1 / M``); ``grad`` is the gradient of ``loss`` with respect to
     the scores before the softcap.
 
-    ``logits`` ``[M, V]`` (fp32, bf16, fp16) are the student's, softcapped at ``cap`` (0: no softcap).
+    ``logits`` ``[M, V]`` (fp32, bf16, fp16; rows of up to 1 MB) are the student's, softcapped at ``cap`` (0: no
+    softcap).
     ``teacher_ids`` (int32 ``[M, K]``, ``K`` up to 1024) and ``teacher_logits`` (fp32, bf16, fp16) are each row's top
     entries of the teacher; its distribution at temperature ``t`` is the softmax over them. An id of -1 is an unused
     place, and a row without entries adds nothing to the KL. Several entries with the same id add up. ``targets``

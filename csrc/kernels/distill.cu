@@ -13,17 +13,23 @@
 // terms after the dense part is written, so every value of dz is rounded once; entries that name the same
 // column add up in the order of their places, so results do not depend on the schedule.
 //
-// The row is read once and kept in registers, as 16-byte vectors of the type it came in: by one block of 256
-// threads up to 16 KB, else by 512 threads per 64 KB in a cluster of up to 8 blocks, which exchange their partial
-// maxima and sums through distributed shared memory; longer rows are read once per pass, again from L2. Bytes
-// bound the call (each logit in and out once); next to that is the exponential unit, 16 results per SM and
-// cycle: a value that both passes need costs two of them. p and P therefore come from one exponential where t is
-// 1 (they are the same) or 2 (exp(x) is the square of exp(x / 2), which doubles a relative error of 2^-22).
+// Persistent blocks, each with every so-manieth row. Three roles run side by side, so that the row's bytes, the
+// entries' chain of dependent loads (ids, then the logits they name) and the arithmetic overlap:
+//   producer warp   bulk copies of the coming rows into a ring in shared memory;
+//   holding warps   a row from the ring into registers (as it came: 16-byte vectors), its sums, and its gradient;
+//   entries' warp   one row ahead: the teacher's distribution, the target, their logits; then the row's loss, and once
+//                   the dense gradient is written the columns that the entries name.
+// Rows of more than 128 KB, and few rows, are split over a cluster of up to 8 blocks, which exchange their partial
+// maxima and sums through distributed shared memory. Bytes bound the call (each logit in and out once); next to
+// that is the exponential unit, 16 results per SM and cycle: a value that both passes need costs two of them. p
+// and P therefore come from one exponential where t is 1 (they are the same) or 2 (exp(x) is the square of
+// exp(x / 2), which doubles a relative error of 2^-22).
 #include <torch/extension.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <atomic>
 #include <string>
 #include <tuple>
 
@@ -33,7 +39,8 @@
 namespace br {
 namespace {
 
-constexpr int kMaxTop = 1024;
+constexpr int kMaxTop = 1024, kMaxTable = 2048;
+constexpr int64_t kMaxRowBytes = 1 << 20;  // 8 blocks of 128 KB
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -46,6 +53,7 @@ enum Mode : int {
 
 struct DistillParams {
   int64_t ld, ldg;  // row strides of the logits and of the gradient
+  int64_t M;
   int V, K;
   const int* ids;  // [M, K]
   const void* teacher;
@@ -55,6 +63,7 @@ struct DistillParams {
   float cap, inv_cap, inv_t, t, alpha, scale;
   int use_cap;     // the softcap bounds the logits: exponentials are taken relative to it, without a maximum
   int cluster;     // blocks of a row
+  int table;       // places of the hash table, a power of two of at least 2 K
   float* rows;     // [M]
   int* status;
 };
@@ -119,246 +128,387 @@ __device__ __forceinline__ float2 peer_pair(const float2* mine, int rank) {
                : "memory");
   return v;
 }
+__device__ __forceinline__ void bulk_row(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 
-// NV > 0: NT x NV vectors per block, kept in registers. NV = 0: any number, read in each pass.
-template <typename T, int NT, int NV, int MODE>
-__global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const T* logits, T* grad, const DistillParams p) {
-  constexpr int E = Vec<T>::E, kHeld = NV > 0 ? NV : 1;
-  extern __shared__ float sm[];  // q [K], l at the ids [K], ids [K]
-  __shared__ float2 red[NT / 32];
-  __shared__ float2 part[2];  // this block's maximum, and its sums; read by the other blocks of the cluster
-  __shared__ float head[6];   // from warp 0: q's part of kl, sum of q, target's logit; target id, entries there
-  float* s_q = sm;
-  float* s_l = sm + p.K;
-  int* s_id = reinterpret_cast<int*>(sm + 2 * p.K);
+constexpr uint64_t kBudgetNs = 2000000000ull;
+
+// NT threads hold NT x NV vectors of a row, S of them wait in the ring; MINB blocks per SM. CAP: cap > 0.
+template <typename T, int NT, int NV, int S, int MINB, int MODE, bool CAP>
+__global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits, T* grad, const DistillParams p) {
+  constexpr int E = Vec<T>::E, kWarps = NT / 32, kPiece = NT * NV;  // vectors of a block
+  constexpr bool kTwoSums = MODE == kSquare || MODE == kHard;
+  extern __shared__ __align__(16) uint8_t smem[];  // [S][kPiece] vectors; two sets of q, l, id [K]; hash table
+  __shared__ uint64_t full[S], empty[S];
+  __shared__ float red[2][2][kWarps], redm[2][kWarps];  // by parity of the row
+  __shared__ float2 part[2], partm[2];                  // this block's sums and maximum, read by the cluster's others
+  __shared__ float s_m[2];
+  __shared__ struct { int some, y; float ly; } info[2];
   asm volatile("griddepcontrol.launch_dependents;");
   const int cs = p.cluster, rank = cs > 1 ? (int)cluster_rank() : 0;
-  const int64_t row = blockIdx.x / cs;
-  const T* L = logits + row * p.ld;
+  const int64_t first = blockIdx.x / cs, stride = gridDim.x / cs;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // the row: edge elements before its first 16-byte boundary, nvec whole vectors, edge elements behind them
-  const int before = (int)((16 - (reinterpret_cast<uintptr_t>(L) & 15)) % 16 / sizeof(T)), n_head = min(before, p.V);
-  const int nvec = (p.V - n_head) / E, tail = n_head + nvec * E;
-  const int edges = n_head + p.V - tail;  // at most 2 (E - 1): one for each of the first threads of the row
-  const bool has_edge = rank == 0 && tid < edges;
-  const int edge_at = tid < n_head ? tid : tail + tid - n_head;
-  const float edge = has_edge ? Vec<T>::one(L[edge_at]) : -INFINITY;
-
-  // vectors of this thread: the v-th is (rank NV + v) NT + tid, or every cs NT-th. f(vector, its first element)
-  uint4 held[kHeld];
-  auto each = [&](auto&& f) {
-    if constexpr (NV > 0) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v) f(held[v], ((rank * NV + v) * NT + tid) * E + n_head);
-    } else {
-      for (int64_t i = (int64_t)rank * NT + tid; i < nvec; i += (int64_t)cs * NT)
-        f(__ldcs(reinterpret_cast<const uint4*>(L + i * E + n_head)), (int)(i * E + n_head));
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kWarps);
     }
-  };
-  if constexpr (NV > 0) {
-    constexpr uint32_t kInf = Vec<T>::kMinusInf;  // no weight in any sum
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = (rank * NV + v) * NT + tid;
-      held[v] = make_uint4(kInf, kInf, kInf, kInf);
-      if (i < nvec) held[v] = __ldcs(reinterpret_cast<const uint4*>(L + (int64_t)i * E + n_head));
-    }
+    fence_barrier_init();
   }
-  // over the row: pairs of sums or maxima, in the order of warps and blocks
-  auto over_row = [&](float a, float b, bool is_max, float2* mine) {
-    a = is_max ? warp_max(a) : warp_sum(a);
-    b = is_max ? b : warp_sum(b);
-    if (lane == 0) red[warp] = make_float2(a, b);
-    __syncthreads();
-    float2 s = red[0];
-#pragma unroll
-    for (int w = 1; w < NT / 32; ++w) s = is_max ? make_float2(fmaxf(s.x, red[w].x), 0.f) : make_float2(s.x + red[w].x, s.y + red[w].y);
-    if (cs > 1) {
-      if (tid == 0) *mine = s;
-      cluster_sync_all();
-      s = peer_pair(mine, 0);
-      for (int r = 1; r < cs; ++r) {
-        const float2 o = peer_pair(mine, r);
-        s = is_max ? make_float2(fmaxf(s.x, o.x), 0.f) : make_float2(s.x + o.x, s.y + o.y);
-      }
-    } else {
-      __syncthreads();  // red is written again
+  __syncthreads();
+  // A wait that runs out records it and goes on, so that every thread still meets every barrier; after the first
+  // failure on the device no further wait spends its budget.
+  auto wait = [&](uint64_t* bar, int64_t phase) {
+    if (!mbar_wait(bar, phase & 1, kBudgetNs, nullptr, p.status)) atomicCAS(p.status, 0, (int)kErrTimeoutProducer);
+  };
+  // a row: edge elements before its first 16-byte boundary, nvec whole vectors, edge elements behind them
+  struct Row {
+    const T* L;
+    int n_head, nvec, tail;
+  };
+  auto row_of = [&](int64_t row) {
+    Row r;
+    r.L = logits + row * p.ld;
+    r.n_head = min((int)((16 - (reinterpret_cast<uintptr_t>(r.L) & 15)) % 16 / sizeof(T)), p.V);
+    r.nvec = (p.V - r.n_head) / E;
+    r.tail = r.n_head + r.nvec * E;
+    return r;
+  };
+  // with max: the cluster's maximum; else its sums. Every thread of the cluster comes here once per row (and kind)
+  auto meet = [&](bool is_max, int par, float2 s) {
+    __syncwarp();
+    cluster_sync_all();
+    const float2* mine = is_max ? &partm[par] : &part[par];
+    s = peer_pair(mine, 0);
+    for (int r = 1; r < cs; ++r) {
+      const float2 o = peer_pair(mine, r);
+      s = is_max ? make_float2(fmaxf(s.x, o.x), 0.f) : make_float2(s.x + o.x, s.y + o.y);
     }
     return s;
   };
-
-  float m = p.cap;
-  if (!p.use_cap) {
-    m = edge;
-    each([&](const uint4& u, int) {
-      float f[E];
-      Vec<T>::unpack(u, f);
-#pragma unroll
-      for (int e = 0; e < E; ++e) m = fmaxf(m, f[e]);
-    });
-    m = over_row(m, 0.f, true, &part[0]).x;
-    if (m == -INFINITY) m = 0.f;  // nothing to take them relative to
-  }
+  const bool need_max = !CAP || !p.use_cap;
   const float k1 = kLog2e * p.inv_t;
-  // exp((l - m) / t) and exp(l - m) of two logits; the difference comes first, so that neither large logits nor
-  // the lowest finite ones lose it
-  const uint64_t m2 = f32x2(m, m), k12 = f32x2(k1, k1), k22 = f32x2(kLog2e, kLog2e);
-  auto soft = [&](float a, float b) {
-    const float2 x = f32x2_split(mul_f32x2(sub_f32x2(f32x2(a, b), m2), k12));
+  const uint64_t k12 = f32x2(k1, k1), k22 = f32x2(kLog2e, kLog2e);
+  // exp((l - m) / t) of two logits, and exp(l - m). Behind a softcap the exponent is one multiply-add (its rounding,
+  // 2^-24 of at most cap / t log2 e, is that small an error of the result); without one the difference comes first,
+  // so that neither large logits nor the lowest finite ones lose it
+  auto power = [&](float a, float b, float m, uint64_t k, float kf) {
+    const uint64_t l = f32x2(a, b);
+    const float2 x = f32x2_split(CAP ? fma_f32x2(l, k, f32x2(-m * kf, -m * kf)) : mul_f32x2(sub_f32x2(l, f32x2(m, m)), k));
     return f32x2(exp2f(x.x), exp2f(x.y));
   };
-  auto hard = [&](float a, float b, uint64_t e) {
-    if constexpr (MODE == kSame) {
-      return e;
-    } else if constexpr (MODE == kSquare) {
-      return mul_f32x2(e, e);
-    } else {
-      const float2 x = f32x2_split(mul_f32x2(sub_f32x2(f32x2(a, b), m2), k22));
-      return f32x2(exp2f(x.x), exp2f(x.y));
-    }
+  auto soft = [&](float a, float b, float m) { return power(a, b, m, k12, k1); };
+  auto hard = [&](float a, float b, float m, uint64_t e) {  // e: soft of the same
+    if constexpr (MODE == kHard) return power(a, b, m, k22, kLog2e);
+    if constexpr (MODE == kSquare) return mul_f32x2(e, e);
+    return e;
   };
+  // a row's factors of the gradient, from its maximum and sums
+  struct Factors {
+    float m, ct, ch, cs1, ch1, loss;
+    bool dead;
+  };
+  auto factors = [&](float m, float2 sums, int some, int y, float ly) {
+    Factors f;
+    const float st = sums.x, s1 = kTwoSums ? sums.y : sums.x;
+    f.m = m;
+    f.dead = st == 0.f;  // every logit is -inf
+    f.ct = f.dead || !some ? 0.f : p.scale * p.alpha * p.t;
+    f.cs1 = f.ct == 0.f ? 0.f : f.ct / st;
+    f.ch = f.ch1 = f.loss = 0.f;
+    if (MODE != kSoft && y >= 0) {
+      const float py = f.dead ? 0.f : f32x2_split(hard(ly, ly, m, soft(ly, ly, m))).x / s1;
+      f.loss = (1.f - p.alpha) * -(log2f(py + 1e-10f) * kLn2);
+      f.ch = p.scale * (1.f - p.alpha) * (py / (py + 1e-10f));
+      f.ch1 = f.dead ? 0.f : f.ch / s1;
+    }
+    return f;
+  };
+  const uint64_t ic2 = f32x2(-p.inv_cap * p.inv_cap, -p.inv_cap * p.inv_cap), one2 = f32x2(1.f, 1.f);
+  // the dense part of the gradient: cs1 exp((l - m) / t) + ch1 exp(l - m), times the softcap's slope (without a softcap
+  // a logit may be -inf, which has none)
+  auto dense = [&](float a, float b, const Factors& f) {
+    const uint64_t x = soft(a, b, f.m), c = f32x2(f.cs1, f.cs1), h = f32x2(f.ch1, f.ch1);
+    if constexpr (MODE == kSoft) return mul_f32x2(c, x);
+    if constexpr (MODE == kSame) return mul_f32x2(f32x2(f.cs1 + f.ch1, f.cs1 + f.ch1), x);
+    if constexpr (MODE == kSquare) return mul_f32x2(x, fma_f32x2(h, x, c));
+    return fma_f32x2(h, hard(a, b, f.m, x), mul_f32x2(c, x));
+  };
+  auto slope = [&](float a, float b) {
+    const uint64_t l = f32x2(a, b);
+    return CAP ? fma_f32x2(mul_f32x2(l, l), ic2, one2) : one2;
+  };
+  auto both = [] {
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(NT + 32) : "memory");
+  };  // holding warps and entries' warp
 
-  if (warp == 0) {
-    // the teacher's distribution over the row's entries, and the target, while the other warps begin their sums
-    float um = -INFINITY;
-    bool some = false;
-    for (int k = lane; k < p.K; k += 32) {
-      const int raw = p.ids[row * p.ld_ids + k];
-      const bool ok = raw == -1 ? false : index_ok(raw, p.V, p.status);
-      const float u = ok ? load_teacher(p, row * p.ld_teacher + k) * p.inv_t : -INFINITY;
-      s_id[k] = ok ? raw : -1;
-      s_q[k] = u;
-      s_l[k] = ok ? Vec<T>::one(L[raw]) : 0.f;
-      um = fmaxf(um, u);
-      some |= u != -INFINITY;
-    }
-    um = warp_max(um);
-    some = __any_sync(0xffffffffu, some);
-    float us = 0.f, a = 0.f, qs = 0.f;
-    if (some)
-      for (int k = lane; k < p.K; k += 32)
-        if (s_id[k] >= 0) us += exp2f((s_q[k] - um) * kLog2e);
-    const float log_us = log2f(warp_sum(us)) * kLn2;
-    for (int k = lane; k < p.K; k += 32) {
-      float q = 0.f;
-      if (some && s_id[k] >= 0) {
-        const float lq = s_q[k] - um - log_us;
-        q = exp2f(lq * kLog2e);
-        if (q != 0.f) a += q * (lq - (s_l[k] - m) * p.inv_t);  // log P = (l - m) / t - log of the row's sum
-        qs += q;
+  if (warp < kWarps) {
+    int n = 0;
+    for (int64_t row = first; row < p.M; row += stride, ++n) {
+      const int par = n & 1;
+      const Row r = row_of(row);
+      // edge elements: one for each of the first threads of the row's first block
+      const bool has_edge = rank == 0 && tid < r.n_head + p.V - r.tail;
+      const int edge_at = tid < r.n_head ? tid : r.tail + tid - r.n_head;
+      const float edge = has_edge ? Vec<T>::one(r.L[edge_at]) : -INFINITY;
+      uint4 held[NV];
+      // each pass unpacks the logits and takes the exponentials anew: kept from the pass before (as the compiler would)
+      // they cost two to four times the registers of the logits as they came
+      auto again = [&] {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) asm volatile("" : "+r"(held[v].x), "+r"(held[v].y), "+r"(held[v].z), "+r"(held[v].w));
+      };
+      const int mine = r.nvec - rank * kPiece - warp * 32;  // vectors of this block from this warp's first on
+      wait(&full[n % S], n / S);
+      {
+        constexpr uint32_t kInf = Vec<T>::kMinusInf;  // no weight in any sum
+        const uint4* ring = reinterpret_cast<const uint4*>(smem) + n % S * kPiece;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          held[v] = make_uint4(kInf, kInf, kInf, kInf);
+          if (v * NT + lane < mine) held[v] = ring[v * NT + tid];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[n % S]);
       }
-      s_q[k] = q;
+      float m = p.cap;
+      if (need_max) {
+        m = edge;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          float f[E];
+          Vec<T>::unpack(held[v], f);
+#pragma unroll
+          for (int e = 0; e < E; ++e) m = fmaxf(m, f[e]);
+        }
+        m = warp_max(m);
+        if (lane == 0) redm[par][warp] = m;
+        asm volatile("bar.sync 2, %0;" ::"n"(NT) : "memory");
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, redm[par][w]);
+        if (cs > 1) {
+          if (tid == 0) partm[par] = make_float2(m, 0.f);
+          m = meet(true, par, make_float2(m, 0.f)).x;
+        }
+        if (m == -INFINITY) m = 0.f;  // nothing to take them relative to
+        again();
+        if (tid == 0) s_m[par] = m;
+      }
+      uint64_t st2 = soft(edge, -INFINITY, m), s12 = 0;
+      if constexpr (kTwoSums) s12 = hard(edge, -INFINITY, m, st2);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        if (v * NT >= mine) break;  // the rest of the warp's vectors are empty
+        float f[E];
+        Vec<T>::unpack(held[v], f);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const uint64_t x = soft(f[e], f[e + 1], m);
+          st2 = add_f32x2(st2, x);
+          if constexpr (MODE == kSquare) s12 = fma_f32x2(x, x, s12);
+          if constexpr (MODE == kHard) s12 = add_f32x2(s12, hard(f[e], f[e + 1], m, x));
+        }
+      }
+      {
+        const float2 a = f32x2_split(st2), b = f32x2_split(s12);
+        const float st = warp_sum(a.x + a.y), s1 = kTwoSums ? warp_sum(b.x + b.y) : 0.f;
+        if (lane == 0) red[par][0][warp] = st, red[par][1][warp] = s1;
+      }
+      both();
+      float2 sums = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) sums = make_float2(sums.x + red[par][0][w], sums.y + red[par][1][w]);
+      if (cs > 1) {
+        if (tid == 0) part[par] = sums;
+        sums = meet(false, par, sums);
+      }
+      if (!grad) continue;
+      const Factors f = factors(m, sums, info[par].some, info[par].y, info[par].ly);
+      T* G = grad + row * p.ldg;
+      const bool aligned = ((reinterpret_cast<uintptr_t>(G) ^ reinterpret_cast<uintptr_t>(r.L)) & 15) == 0;
+      again();
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        if (v * NT >= mine) break;
+        float x[E];
+        Vec<T>::unpack(held[v], x);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          uint64_t g = dense(x[e], x[e + 1], f);
+          if constexpr (CAP) g = mul_f32x2(g, slope(x[e], x[e + 1]));
+          const float2 o = f32x2_split(g);
+          x[e] = o.x;
+          x[e + 1] = o.y;
+        }
+        if (v * NT + lane < mine) store_vec(G + r.n_head + (int64_t)(rank * kPiece + v * NT + tid) * E, aligned, x);
+      }
+      if (has_edge) {
+        const float g = f32x2_split(dense(edge, edge, f)).x;
+        G[edge_at] = Vec<T>::round(CAP ? g * f32x2_split(slope(edge, edge)).x : g);
+      }
     }
-    a = warp_sum(a);
-    qs = warp_sum(qs);
-    if (lane == 0) {
+    both();  // the last row's gradient is written
+  } else if (warp == kWarps) {
+    float* ent_mem = reinterpret_cast<float*>(smem + (size_t)S * kPiece * 16);
+    int* table = reinterpret_cast<int*>(ent_mem + 6 * p.K);
+    auto q_of = [&](int par) { return ent_mem + 3 * p.K * par; };
+    // the columns that the entries and the target of a row name, once its dense gradient is written
+    auto patch = [&](int64_t row, int par, const Factors& f, int y, float ly) {
+      if (!grad || f.dead) return;
+      const float *s_q = q_of(par), *s_l = s_q + p.K;
+      const int* s_id = reinterpret_cast<const int*>(s_l + p.K);
+      const Row r = row_of(row);
+      T* G = grad + row * p.ldg;
+      for (int k = lane; k < p.K + (MODE != kSoft ? 1 : 0); k += 32) {
+        const int id = k < p.K ? s_id[k] : y;
+        if (id < 0) continue;
+        const int by = id < r.n_head || id >= r.tail ? 0 : (id - r.n_head) / E / kPiece;  // the block that has the column
+        if (by != rank) continue;
+        const float l = k < p.K ? s_l[k] : ly;
+        float q = k < p.K ? s_q[k] : 0.f;
+        if (k == p.K) {  // the target's own column: an entry that names it has all the column's mass
+          for (int i = 0; i < p.K; ++i)
+            if (s_id[i] == id) q = s_q[i];
+        }
+        float g = f32x2_split(dense(l, l, f)).x - f.ct * q;
+        if (MODE != kSoft && id == y) g -= f.ch;
+        G[id] = Vec<T>::round(g * f32x2_split(slope(l, l)).x);
+      }
+      __syncwarp();
+    };
+    int n = 0;
+    Factors last{};
+    int last_y = -1;
+    float last_ly = 0.f;
+    for (int64_t row = first; row < p.M; row += stride, ++n) {
+      const int par = n & 1;
+      // ---- prepare this row's entries
+      float *s_q = q_of(par), *s_l = s_q + p.K;
+      int* s_id = reinterpret_cast<int*>(s_l + p.K);
+      const T* L = logits + row * p.ld;
       int y = -1;
+      float ly = 0.f;
       if constexpr (MODE != kSoft) {
         y = p.targets[row];
         if (y != -1 && !index_ok(y, p.V, p.status)) y = -1;
+        ly = y >= 0 ? Vec<T>::one(L[y]) : 0.f;
       }
-      head[0] = a;
-      head[1] = qs;
-      head[2] = y >= 0 ? Vec<T>::one(L[y]) : 0.f;
-      head[3] = __int_as_float(y);
-      head[4] = some ? 1.f : 0.f;
-    }
-  }
-  uint64_t st2 = soft(edge, -INFINITY), s12 = 0;
-  if constexpr (MODE != kSoft) s12 = hard(edge, -INFINITY, st2);
-  each([&](const uint4& u, int) {
-    float f[E];
-    Vec<T>::unpack(u, f);
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const uint64_t x = soft(f[e], f[e + 1]);
-      st2 = add_f32x2(st2, x);
-      if constexpr (MODE != kSoft) s12 = add_f32x2(s12, hard(f[e], f[e + 1], x));
-    }
-  });
-  float st = f32x2_split(st2).x + f32x2_split(st2).y, s1 = f32x2_split(s12).x + f32x2_split(s12).y;
-  // in place too: every block of the row has read the columns that the teacher and the target name
-  const float2 sums = over_row(st, s1, false, &part[1]);
-  if (cs > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // the others' sums are read
-  st = sums.x;
-  s1 = sums.y;
-  const bool dead = st == 0.f, some = head[4] != 0.f;
-  float py = 0.f, r = 0.f, loss = 0.f;
-  if (some) loss = dead ? INFINITY : p.alpha * p.t * p.t * fmaf(log2f(st) * kLn2, head[1], head[0]);
-  if (p.alpha == 0.f) loss = 0.f;
-  const int y = __float_as_int(head[3]);
-  const float ly = head[2];
-  if constexpr (MODE != kSoft) {
-    if (y >= 0) {
-      py = dead ? 0.f : f32x2_split(hard(ly, ly, soft(ly, ly))).x / s1;
-      loss += (1.f - p.alpha) * -(log2f(py + 1e-10f) * kLn2);
-      r = (1.f - p.alpha) * (py / (py + 1e-10f));
-    }
-  }
-  if (tid == 0 && rank == 0) p.rows[row] = loss;
-  if (grad) {
-    T* G = grad + row * p.ldg;
-    const bool aligned = ((reinterpret_cast<uintptr_t>(G) ^ reinterpret_cast<uintptr_t>(L)) & 15) == 0;
-    const float ct = dead || !some ? 0.f : p.scale * p.alpha * p.t, cs1 = ct == 0.f ? 0.f : ct / st;
-    const float ch = dead ? 0.f : p.scale * r, ch1 = ch == 0.f ? 0.f : ch / s1;
-    const uint64_t cs12 = f32x2(cs1, cs1), ch12 = f32x2(ch1, ch1);
-    auto dense = [&](float a, float b) {
-      const uint64_t x = soft(a, b);
-      uint64_t g = mul_f32x2(cs12, x);
-      if constexpr (MODE != kSoft) g = fma_f32x2(ch12, hard(a, b, x), g);
-      return g;
-    };
-    if constexpr (NV > 0) {
-      // the exponentials are taken again: kept from the first pass they would cost twice the logits' registers
-#pragma unroll
-      for (int v = 0; v < NV; ++v) asm volatile("" : "+r"(held[v].x), "+r"(held[v].y), "+r"(held[v].z), "+r"(held[v].w));
-    }
-    const uint64_t ic2 = f32x2(p.inv_cap, p.inv_cap), one2 = f32x2(1.f, 1.f);
-    auto write = [&](auto capped) {
-      auto slope = [&](float a, float b, uint64_t g) {
-        if constexpr (decltype(capped)::value) {
-          const uint64_t c = mul_f32x2(f32x2(a, b), ic2);
-          g = mul_f32x2(g, sub_f32x2(one2, mul_f32x2(c, c)));
-        }
-        return g;
-      };
-      each([&](const uint4& u, int e0) {
-        float f[E];
-        Vec<T>::unpack(u, f);
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          const float2 o = f32x2_split(slope(f[e], f[e + 1], dense(f[e], f[e + 1])));
-          f[e] = o.x;
-          f[e + 1] = o.y;
-        }
-        if (e0 < tail) store_vec(G + e0, aligned, f);
-      });
-      if (has_edge) G[edge_at] = Vec<T>::round(f32x2_split(slope(edge, edge, dense(edge, edge))).x);
-    };
-    if (p.inv_cap > 0.f) {
-      write(std::true_type{});
-    } else {
-      write(std::false_type{});  // a logit may be -inf, which has no slope
-    }
-    __syncthreads();
-    if (!dead) {
-      for (int k = tid; k < p.K + (MODE != kSoft ? 1 : 0); k += NT) {
-        const int id = k < p.K ? s_id[k] : y;
-        if (id < 0) continue;
-        const int vec = (id - n_head) / E;  // the block that wrote the column, of the row's blocks
-        const int by = id < n_head || id >= tail ? 0 : NV > 0 ? vec / (NT * kHeld) : vec / NT % cs;
-        if (by != rank) continue;
-        const float l = k < p.K ? s_l[k] : ly;
+      float um = -INFINITY, lm = -INFINITY;
+      bool some = false;
+      for (int k = lane; k < p.K; k += 32) {
+        const int raw = p.ids[row * p.ld_ids + k];
+        const float teacher = load_teacher(p, row * p.ld_teacher + k);
+        const bool ok = raw == -1 ? false : index_ok(raw, p.V, p.status);
+        const float u = ok ? teacher * p.inv_t : -INFINITY;
+        const float l = ok ? Vec<T>::one(L[raw]) : -INFINITY;
+        s_id[k] = ok ? raw : -1;
+        s_q[k] = u;
+        s_l[k] = l;
+        um = fmaxf(um, u);
+        lm = fmaxf(lm, l);
+        some |= u != -INFINITY;
+      }
+      um = warp_max(um);
+      lm = warp_max(lm);
+      if (lm == -INFINITY) lm = 0.f;
+      some = __any_sync(0xffffffffu, some);
+      float us = 0.f;
+      if (some)
+        for (int k = lane; k < p.K; k += 32)
+          if (s_id[k] >= 0) us += exp2f((s_q[k] - um) * kLog2e);
+      const float log_us = log2f(warp_sum(us)) * kLn2;
+      // kl = sum of q (log q - (l - lm) / t) + sum of q ((m - lm) / t + log of the row's sum)
+      float ent = 0.f, qs = 0.f;
+      for (int k = lane; k < p.K; k += 32) {
         float q = 0.f;
-        for (int i = 0; i < p.K; ++i) q += s_id[i] == id ? s_q[i] : 0.f;
-        float g = f32x2_split(dense(l, l)).x - ct * q;
-        if (MODE != kSoft && id == y) g -= ch;
-        const float c = p.inv_cap > 0.f ? l * p.inv_cap : 0.f;
-        G[id] = Vec<T>::round(g * fmaf(-c, c, 1.f));
+        if (some && s_id[k] >= 0) {
+          const float lq = s_q[k] - um - log_us;
+          q = exp2f(lq * kLog2e);
+          if (q != 0.f) ent += q * (lq - (s_l[k] - lm) * p.inv_t);
+          qs += q;
+        }
+        s_q[k] = q;
       }
+      ent = warp_sum(ent);
+      qs = warp_sum(qs);
+      // do two entries name the same column? each id goes into an open-addressed table, where it meets its like
+      bool twice = false;
+      for (int k = lane; k < p.table; k += 32) table[k] = -1;
+      __syncwarp();
+      for (int k = lane; k < p.K; k += 32) {
+        const int id = s_id[k];
+        if (id < 0) continue;
+        for (int at = (int)((uint32_t)id * 2654435761u >> 7) & (p.table - 1);; at = (at + 1) & (p.table - 1)) {
+          const int was = atomicCAS(&table[at], -1, id);
+          twice |= was == id;
+          if (was == -1 || was == id) break;  // at most half of the places are taken
+        }
+      }
+      __syncwarp();
+      if (__any_sync(0xffffffffu, twice)) {
+        // give each entry the mass of all that name its column, added in the order of their places
+        for (int k = lane; k < p.K; k += 32) {
+          float q = 0.f;
+          for (int i = 0; i < p.K; ++i) q += s_id[i] == s_id[k] ? s_q[i] : 0.f;
+          reinterpret_cast<float*>(table)[k] = q;
+        }
+        __syncwarp();
+        for (int k = lane; k < p.K; k += 32) s_q[k] = reinterpret_cast<float*>(table)[k];
+      }
+      if (lane == 0) info[par].some = some, info[par].y = y, info[par].ly = ly;
+      __syncwarp();
+      // ---- the row's sums; the row before is written
+      if (need_max && cs > 1) meet(true, par, make_float2(0.f, 0.f));
+      both();
+      float2 sums = make_float2(0.f, 0.f);
+      for (int w = 0; w < kWarps; ++w) sums = make_float2(sums.x + red[par][0][w], sums.y + red[par][1][w]);
+      if (cs > 1) sums = meet(false, par, sums);
+      const float m = need_max ? s_m[par] : p.cap;
+      const Factors f = factors(m, sums, some, y, ly);
+      if (lane == 0 && rank == 0) {
+        float loss = f.loss;
+        if (some && p.alpha != 0.f)
+          loss += f.dead ? INFINITY : p.alpha * p.t * p.t * fmaf((m - lm) * p.inv_t + log2f(sums.x) * kLn2, qs, ent);
+        p.rows[row] = loss;
+      }
+      if (n > 0) patch(row - stride, par ^ 1, last, last_y, last_ly);
+      last = f;
+      last_y = y;
+      last_ly = ly;
+    }
+    both();
+    if (n > 0) patch(first + (n - 1) * stride, (n - 1) & 1, last, last_y, last_ly);
+  } else {
+    // the producer: this block's whole vectors of each row, S rows ahead
+    auto load = [&](int64_t row, int n) {
+      const Row r = row_of(row);
+      const int count = max(0, min(r.nvec - rank * kPiece, kPiece));
+      mbar_arrive_expect_tx(&full[n % S], count * 16);
+      if (count > 0)
+        bulk_row(smem + (size_t)(n % S) * kPiece * 16, r.L + r.n_head + (int64_t)rank * kPiece * E, count * 16, &full[n % S]);
+    };
+    if (lane == 0)
+      for (int n = 0; n < S; ++n)
+        if (first + n * stride < p.M) load(first + n * stride, n);
+    int n = 0;
+    for (int64_t row = first; row < p.M; row += stride, ++n) {
+      if (cs > 1) {
+        if (need_max) cluster_sync_all();
+        cluster_sync_all();
+      }
+      if (lane == 0 && row + S * stride < p.M) {
+        wait(&empty[n % S], n / S);
+        load(row + S * stride, n + S);
+      }
+      __syncwarp();
     }
   }
-  if (cs > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // shared memory stays until then
+  if (cs > 1) cluster_sync_all();  // the others may still read this block's sums
 }
 
 // loss = scale * sum of the rows, in one fixed order: one block, each thread's rows in order in 64 bits. Launched
@@ -384,6 +534,17 @@ void by_float(at::ScalarType t, F&& f) {
   if (t == at::kFloat) return f(float{});
   if (t == at::kBFloat16) return f(__nv_bfloat16{});
   f(__half{});
+}
+
+// a kernel's attributes belong to a device: f runs once for each device that the kernel is used on
+template <auto kernel, typename F>
+void once_per_device(int device, F&& f) {
+  static std::atomic<uint64_t> done{0};
+  TORCH_CHECK(device >= 0 && device < 64, "bad device index");
+  if (!(done.load(std::memory_order_acquire) >> device & 1)) {
+    f();
+    done.fetch_or(uint64_t(1) << device, std::memory_order_release);
+  }
 }
 
 // a launch with cluster blocks per cluster, or as a dependent of the launch before it
@@ -412,22 +573,50 @@ void launch(void (*kernel)(P...), int64_t blocks, int threads, size_t smem, cuda
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
 }
 
-template <typename T, int MODE>
-void launch_rows(int64_t M, int64_t V, const T* logits, T* grad, DistillParams& p, int sms, cudaStream_t st) {
-  const int64_t vecs = std::max<int64_t>(1, V / Vec<T>::E);
-  const size_t smem = (size_t)p.K * 12;
-  // a row's blocks: as few as hold it; more while the GPU has SMs to spare and each keeps 256 vectors (4 KB)
+template <typename T, int NT, int NV, int S, int MINB, int MODE, bool CAP>
+void launch_held(const T* logits, T* grad, const DistillParams& p, int device, int sms, cudaStream_t st) {
+  auto* kernel = distill_kernel<T, NT, NV, S, MINB, MODE, CAP>;
+  const size_t smem = (size_t)S * NT * NV * 16 + (size_t)p.K * 24 + (size_t)p.table * 4;
+  once_per_device<distill_kernel<T, NT, NV, S, MINB, MODE, CAP>>(device, [&] {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        S * NT * NV * 16 + kMaxTop * 24 + kMaxTable * 4));
+  });
+  // persistent: as many blocks as run at once, whole clusters, no more than rows
+  const int64_t groups = std::max<int64_t>(1, (int64_t)sms * MINB / p.cluster);
+  launch(kernel, std::min<int64_t>(p.M, groups) * p.cluster, NT + 64, smem, st, p.cluster, false, logits, grad, p);
+}
+
+template <typename T, int MODE, bool CAP>
+void launch_rows(const T* logits, T* grad, DistillParams& p, int device, int sms, cudaStream_t st) {
+  const int64_t vecs = std::max(1, p.V / Vec<T>::E);
+  // a row's blocks: as few as hold it in 128 KB each; more while the GPU has SMs to spare and each keeps 512 vectors (8 KB)
   p.cluster = 1;
-  while (p.cluster < 8 && (vecs > p.cluster * 4096 || (M * p.cluster * 2 <= sms && vecs > p.cluster * 512))) p.cluster *= 2;
-  const int64_t blocks = M * p.cluster;
-  TORCH_CHECK_VALUE(blocks < (int64_t(1) << 31), "distill_topk: too many rows");
-  if (vecs <= p.cluster * 1024) {
-    launch(distill_kernel<T, 256, 4, MODE>, blocks, 256, smem, st, p.cluster, false, logits, grad, p);
-  } else if (vecs <= p.cluster * 4096) {
-    launch(distill_kernel<T, 512, 8, MODE>, blocks, 512, smem, st, p.cluster, false, logits, grad, p);
-  } else {
-    launch(distill_kernel<T, 512, 0, MODE>, blocks, 512, smem, st, p.cluster, false, logits, grad, p);
+  while (p.cluster < 8 && (vecs > p.cluster * 8192 || (p.M * p.cluster * 2 <= sms && vecs > p.cluster * 1024)))
+    p.cluster *= 2;
+  if (vecs <= p.cluster * 1024) {  // 16 KB per block
+    launch_held<T, 256, 4, 3, 4, MODE, CAP>(logits, grad, p, device, sms, st);
+  } else if (vecs <= p.cluster * 4096) {  // 64 KB
+    launch_held<T, 512, 8, 1, 2, MODE, CAP>(logits, grad, p, device, sms, st);
+  } else {  // 128 KB
+    launch_held<T, 512, 16, 1, 1, MODE, CAP>(logits, grad, p, device, sms, st);
   }
+}
+
+template <typename T>
+void launch_rows_mode(bool hard, const T* logits, T* grad, DistillParams& p, int device, int sms, cudaStream_t st) {
+  auto with = [&](auto cap) {
+    constexpr bool C = decltype(cap)::value;
+    if (!hard) {
+      launch_rows<T, kSoft, C>(logits, grad, p, device, sms, st);
+    } else if (p.t == 1.f) {
+      launch_rows<T, kSame, C>(logits, grad, p, device, sms, st);
+    } else if (p.t == 2.f) {
+      launch_rows<T, kSquare, C>(logits, grad, p, device, sms, st);
+    } else {
+      launch_rows<T, kHard, C>(logits, grad, p, device, sms, st);
+    }
+  };
+  p.cap > 0 ? with(std::true_type{}) : with(std::false_type{});
 }
 
 }  // namespace
@@ -442,7 +631,9 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> distill_t
   };
   TORCH_CHECK_VALUE(logits.dim() == 2 && real(logits), what, "logits must be [M, V] in float32, bfloat16 or float16");
   const int64_t M = logits.size(0), V = logits.size(1);
-  TORCH_CHECK_VALUE(V >= 1 && V < (int64_t(1) << 30) && M < (int64_t(1) << 31), what, "logits out of range");
+  TORCH_CHECK_VALUE(V >= 1 && M < (int64_t(1) << 31), what, "logits out of range");
+  TORCH_CHECK_VALUE(V * logits.element_size() <= kMaxRowBytes, what, "rows of the logits of up to 1 MB, got ",
+                    std::to_string(V * logits.element_size()), " bytes");
   TORCH_CHECK_VALUE(V == 1 || logits.stride(1) == 1, what, "logits need contiguous rows");
   TORCH_CHECK_VALUE(M <= 1 || logits.stride(0) >= V, what, "rows of the logits overlap");
   TORCH_CHECK_VALUE(ids.dim() == 2 && ids.size(0) == M && ids.scalar_type() == at::kInt, what,
@@ -493,6 +684,7 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> distill_t
   DistillParams p{};
   p.ld = M > 1 ? logits.stride(0) : V;
   p.ldg = need_grad && M > 1 ? grad->stride(0) : V;
+  p.M = M;
   p.V = (int)V;
   p.K = (int)K;
   p.ids = ids.data_ptr<int>();
@@ -509,6 +701,8 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> distill_t
   p.scale = (float)scale;
   // exponentials relative to the softcap span e^(-2 cap / t): far above fp32's smallest number up to 2 cap / t = 60
   p.use_cap = cap > 0 && 2 * cap <= 60 * std::min(1.0, temperature);
+  p.table = 32;
+  while (p.table < 2 * p.K) p.table *= 2;
   p.rows = rows.data_ptr<float>();
   p.status = status_ptr(logits.device().index());
   if (M > 0) {
@@ -518,15 +712,7 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> distill_t
       using T = decltype(lt);
       const T* l = reinterpret_cast<const T*>(logits.data_ptr());
       T* dz = need_grad ? reinterpret_cast<T*>(grad->data_ptr()) : nullptr;
-      if (!hard) {
-        launch_rows<T, kSoft>(M, V, l, dz, p, sms, st);
-      } else if (p.t == 1.f) {
-        launch_rows<T, kSame>(M, V, l, dz, p, sms, st);
-      } else if (p.t == 2.f) {
-        launch_rows<T, kSquare>(M, V, l, dz, p, sms, st);
-      } else {
-        launch_rows<T, kHard>(M, V, l, dz, p, sms, st);
-      }
+      launch_rows_mode<T>(hard, l, dz, p, logits.device().index(), sms, st);
     });
   }
   launch(sum_rows_kernel, 1, kSumThreads, 0, st, 1, M > 0, rows.data_ptr<float>(), M, p.scale, loss.data_ptr<float>());

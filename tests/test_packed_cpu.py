@@ -136,6 +136,7 @@ def test_bounds_refuse():
 @pytest.mark.parametrize("change,message", [
     (lambda a: a.update(logits=a["logits"].double()), "logits must be"),
     (lambda a: a.update(logits=torch.zeros(9, 4).t()), "contiguous rows"),
+    (lambda a: a.update(logits=torch.zeros(4, (1 << 18) + 1)), "up to 1 MB"),
     (lambda a: a.update(logits=torch.zeros(1, 9).expand(4, 9)), "overlap"),
     (lambda a: a.update(teacher_ids=a["teacher_ids"].long()), "teacher_ids must be int32"),
     (lambda a: a.update(teacher_ids=a["teacher_ids"][:3]), "teacher_ids must be int32"),
