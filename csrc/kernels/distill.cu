@@ -17,8 +17,9 @@
 // entries' chain of dependent loads (ids, then the logits they name) and the arithmetic overlap:
 //   producer warp   bulk copies of the coming rows into a ring in shared memory;
 //   holding warps   a row from the ring into registers (as it came: 16-byte vectors), its sums, and its gradient;
-//   entries' warp   one row ahead: the teacher's distribution, the target, their logits; then the row's loss, and once
-//                   the dense gradient is written the columns that the entries name.
+//   entries' warps  taking the rows in turn, so that each has several rows' time: the teacher's distribution, the target,
+//                   their logits; then the row's loss, and once the dense gradient is written the columns that
+//                   the entries name.
 // Rows of more than 128 KB, and few rows, are split over a cluster of up to 8 blocks, which exchange their partial
 // maxima and sums through distributed shared memory. Bytes bound the call (each logit in and out once); next to
 // that is the exponential unit, 16 results per SM and cycle: a value that both passes need costs two of them. p
@@ -137,17 +138,18 @@ __device__ __forceinline__ void bulk_row(void* dst, const void* src, uint32_t by
 
 constexpr uint64_t kBudgetNs = 2000000000ull;
 
-// NT threads hold NT x NV vectors of a row, S of them wait in the ring; MINB blocks per SM. CAP: cap > 0.
-template <typename T, int NT, int NV, int S, int MINB, int MODE, bool CAP>
-__global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits, T* grad, const DistillParams p) {
+// NT threads hold NT x NV vectors of a row, S of them wait in the ring, TW warps see to the entries; MINB blocks per
+// SM. CAP: cap > 0.
+template <typename T, int NT, int NV, int S, int TW, int MINB, int MODE, bool CAP>
+__global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const T* logits, T* grad, const DistillParams p) {
   constexpr int E = Vec<T>::E, kWarps = NT / 32, kPiece = NT * NV;  // vectors of a block
   constexpr bool kTwoSums = MODE == kSquare || MODE == kHard;
-  extern __shared__ __align__(16) uint8_t smem[];  // [S][kPiece] vectors; two sets of q, l, id [K]; hash table
-  __shared__ uint64_t full[S], empty[S];
+  extern __shared__ __align__(16) uint8_t smem[];  // [S][kPiece] vectors; per entries' warp q, l, id [K] and a hash table
+  __shared__ uint64_t full[S], empty[S], written[TW];
   __shared__ float red[2][2][kWarps], redm[2][kWarps];  // by parity of the row
   __shared__ float2 part[2], partm[2];                  // this block's sums and maximum, read by the cluster's others
   __shared__ float s_m[2];
-  __shared__ struct { int some, y; float ly; } info[2];
+  __shared__ struct { int some, y; float ly; } info[TW];
   asm volatile("griddepcontrol.launch_dependents;");
   const int cs = p.cluster, rank = cs > 1 ? (int)cluster_rank() : 0;
   const int64_t first = blockIdx.x / cs, stride = gridDim.x / cs;
@@ -157,6 +159,7 @@ __global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits,
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], kWarps);
     }
+    for (int i = 0; i < TW; ++i) mbar_init(&written[i], kWarps);
     fence_barrier_init();
   }
   __syncthreads();
@@ -242,9 +245,10 @@ __global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits,
     const uint64_t l = f32x2(a, b);
     return CAP ? fma_f32x2(mul_f32x2(l, l), ic2, one2) : one2;
   };
-  auto both = [] {
+  // the holding warps and the entries' warp of row n: its sums and its entries are there
+  auto both = [](int n) {
     __syncwarp();
-    asm volatile("bar.sync 1, %0;" ::"n"(NT + 32) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(2 + n % TW), "n"(NT + 32) : "memory");
   };  // holding warps and entries' warp
 
   if (warp < kWarps) {
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits,
         }
         m = warp_max(m);
         if (lane == 0) redm[par][warp] = m;
-        asm volatile("bar.sync 2, %0;" ::"n"(NT) : "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) m = fmaxf(m, redm[par][w]);
         if (cs > 1) {
@@ -319,7 +323,7 @@ __global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits,
         const float st = warp_sum(a.x + a.y), s1 = kTwoSums ? warp_sum(b.x + b.y) : 0.f;
         if (lane == 0) red[par][0][warp] = st, red[par][1][warp] = s1;
       }
-      both();
+      both(n);
       float2 sums = make_float2(0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) sums = make_float2(sums.x + red[par][0][w], sums.y + red[par][1][w]);
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits,
         sums = meet(false, par, sums);
       }
       if (!grad) continue;
-      const Factors f = factors(m, sums, info[par].some, info[par].y, info[par].ly);
+      const Factors f = factors(m, sums, info[n % TW].some, info[n % TW].y, info[n % TW].ly);
       T* G = grad + row * p.ldg;
       const bool aligned = ((reinterpret_cast<uintptr_t>(G) ^ reinterpret_cast<uintptr_t>(r.L)) & 15) == 0;
       again();
@@ -351,17 +355,18 @@ __global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits,
         const float g = f32x2_split(dense(edge, edge, f)).x;
         G[edge_at] = Vec<T>::round(CAP ? g * f32x2_split(slope(edge, edge)).x : g);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&written[n % TW]);
     }
-    both();  // the last row's gradient is written
-  } else if (warp == kWarps) {
-    float* ent_mem = reinterpret_cast<float*>(smem + (size_t)S * kPiece * 16);
-    int* table = reinterpret_cast<int*>(ent_mem + 6 * p.K);
-    auto q_of = [&](int par) { return ent_mem + 3 * p.K * par; };
+  } else if (warp < kWarps + TW) {
+    const int turn = warp - kWarps;
+    float* s_q = reinterpret_cast<float*>(smem + (size_t)S * kPiece * 16) + (3 * p.K + p.table) * turn;
+    float* s_l = s_q + p.K;
+    int* s_id = reinterpret_cast<int*>(s_l + p.K);
+    int* table = s_id + p.K;
     // the columns that the entries and the target of a row name, once its dense gradient is written
-    auto patch = [&](int64_t row, int par, const Factors& f, int y, float ly) {
-      if (!grad || f.dead) return;
-      const float *s_q = q_of(par), *s_l = s_q + p.K;
-      const int* s_id = reinterpret_cast<const int*>(s_l + p.K);
+    auto patch = [&](int64_t row, const Factors& f, int y, float ly) {
+      if (f.dead) return;
       const Row r = row_of(row);
       T* G = grad + row * p.ldg;
       for (int k = lane; k < p.K + (MODE != kSoft ? 1 : 0); k += 32) {
@@ -382,14 +387,16 @@ __global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits,
       __syncwarp();
     };
     int n = 0;
-    Factors last{};
-    int last_y = -1;
-    float last_ly = 0.f;
     for (int64_t row = first; row < p.M; row += stride, ++n) {
       const int par = n & 1;
-      // ---- prepare this row's entries
-      float *s_q = q_of(par), *s_l = s_q + p.K;
-      int* s_id = reinterpret_cast<int*>(s_l + p.K);
+      if (n % TW != turn) {
+        if (cs > 1) {  // every thread of the cluster meets
+          if (need_max) meet(true, par, make_float2(0.f, 0.f));
+          meet(false, par, make_float2(0.f, 0.f));
+        }
+        continue;
+      }
+      // ---- the row's entries
       const T* L = logits + row * p.ld;
       int y = -1;
       float ly = 0.f;
@@ -460,11 +467,10 @@ __global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits,
         __syncwarp();
         for (int k = lane; k < p.K; k += 32) s_q[k] = reinterpret_cast<float*>(table)[k];
       }
-      if (lane == 0) info[par].some = some, info[par].y = y, info[par].ly = ly;
-      __syncwarp();
-      // ---- the row's sums; the row before is written
+      if (lane == 0) info[turn].some = some, info[turn].y = y, info[turn].ly = ly;
+      // ---- its sums
       if (need_max && cs > 1) meet(true, par, make_float2(0.f, 0.f));
-      both();
+      both(n);
       float2 sums = make_float2(0.f, 0.f);
       for (int w = 0; w < kWarps; ++w) sums = make_float2(sums.x + red[par][0][w], sums.y + red[par][1][w]);
       if (cs > 1) sums = meet(false, par, sums);
@@ -476,13 +482,11 @@ __global__ void __launch_bounds__(NT + 64, MINB) distill_kernel(const T* logits,
           loss += f.dead ? INFINITY : p.alpha * p.t * p.t * fmaf((m - lm) * p.inv_t + log2f(sums.x) * kLn2, qs, ent);
         p.rows[row] = loss;
       }
-      if (n > 0) patch(row - stride, par ^ 1, last, last_y, last_ly);
-      last = f;
-      last_y = y;
-      last_ly = ly;
+      if (grad) {
+        wait(&written[turn], n / TW);
+        patch(row, f, y, ly);
+      }
     }
-    both();
-    if (n > 0) patch(first + (n - 1) * stride, (n - 1) & 1, last, last_y, last_ly);
   } else {
     // the producer: this block's whole vectors of each row, S rows ahead
     auto load = [&](int64_t row, int n) {
@@ -573,17 +577,17 @@ void launch(void (*kernel)(P...), int64_t blocks, int threads, size_t smem, cuda
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
 }
 
-template <typename T, int NT, int NV, int S, int MINB, int MODE, bool CAP>
+template <typename T, int NT, int NV, int S, int TW, int MINB, int MODE, bool CAP>
 void launch_held(const T* logits, T* grad, const DistillParams& p, int device, int sms, cudaStream_t st) {
-  auto* kernel = distill_kernel<T, NT, NV, S, MINB, MODE, CAP>;
-  const size_t smem = (size_t)S * NT * NV * 16 + (size_t)p.K * 24 + (size_t)p.table * 4;
-  once_per_device<distill_kernel<T, NT, NV, S, MINB, MODE, CAP>>(device, [&] {
+  auto* kernel = distill_kernel<T, NT, NV, S, TW, MINB, MODE, CAP>;
+  const size_t smem = (size_t)S * NT * NV * 16 + TW * ((size_t)p.K * 12 + (size_t)p.table * 4);
+  once_per_device<distill_kernel<T, NT, NV, S, TW, MINB, MODE, CAP>>(device, [&] {
     C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        S * NT * NV * 16 + kMaxTop * 24 + kMaxTable * 4));
+                                        S * NT * NV * 16 + TW * (kMaxTop * 12 + kMaxTable * 4)));
   });
   // persistent: as many blocks as run at once, whole clusters, no more than rows
   const int64_t groups = std::max<int64_t>(1, (int64_t)sms * MINB / p.cluster);
-  launch(kernel, std::min<int64_t>(p.M, groups) * p.cluster, NT + 64, smem, st, p.cluster, false, logits, grad, p);
+  launch(kernel, std::min<int64_t>(p.M, groups) * p.cluster, NT + 32 * TW + 32, smem, st, p.cluster, false, logits, grad, p);
 }
 
 template <typename T, int MODE, bool CAP>
@@ -594,11 +598,11 @@ void launch_rows(const T* logits, T* grad, DistillParams& p, int device, int sms
   while (p.cluster < 8 && (vecs > p.cluster * 8192 || (p.M * p.cluster * 2 <= sms && vecs > p.cluster * 1024)))
     p.cluster *= 2;
   if (vecs <= p.cluster * 1024) {  // 16 KB per block
-    launch_held<T, 256, 4, 3, 4, MODE, CAP>(logits, grad, p, device, sms, st);
+    launch_held<T, 128, 8, 3, 3, 4, MODE, CAP>(logits, grad, p, device, sms, st);
   } else if (vecs <= p.cluster * 4096) {  // 64 KB
-    launch_held<T, 512, 8, 1, 2, MODE, CAP>(logits, grad, p, device, sms, st);
+    launch_held<T, 512, 8, 2, 2, 1, MODE, CAP>(logits, grad, p, device, sms, st);
   } else {  // 128 KB
-    launch_held<T, 512, 16, 1, 1, MODE, CAP>(logits, grad, p, device, sms, st);
+    launch_held<T, 512, 16, 1, 2, 1, MODE, CAP>(logits, grad, p, device, sms, st);
   }
 }
 
