@@ -56,7 +56,7 @@ struct PackedParams {
   const int* start;
   const int* end;
   float* lse;    // [H, N], natural log
-  float2* stat;  // backward scratch [H, Np]: (lse in log2 units, delta) of each row; (inf, 0) for rows of no sequence
+  float2* stat;  // backward scratch [H, Np]: (-lse in log2 units, -delta) of each row; (-inf, 0) for rows of no sequence
   int Np;        // N rounded up to whole tiles
 };
 
@@ -188,8 +188,8 @@ __device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool w
         load_row<T, D>(p.q, i, h, lane, q);
         load_row<T, D>(p.dout, i, h, lane, d);
         const float2 st = stat[i];
-        const float w = exp2f(dot(q, k) * p.scale_log2 - st.x);
-        const float ds = w * (dot(d, v) - st.y);
+        const float w = exp2f(dot(q, k) * p.scale_log2 + st.x);
+        const float ds = w * (dot(d, v) + st.y);
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = i0 + u < hi ? fmaf(want_dk ? ds : w, want_dk ? q[e] : d[e], acc[e]) : acc[e];
       }
@@ -203,7 +203,7 @@ __device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool w
 }
 
 // ---------------------------------------------------------------------------------------- forward, tcgen05
-// Persistent, one CTA per SM, 320 threads. A work item is two 128-row query tiles A and B that share their keys: two
+// Persistent, one CTA per SM, 384 threads. A work item is two 128-row query tiles A and B that share their keys: two
 // heads of one kv head over the same rows where the group of query heads is even, else two neighbouring row
 // tiles of one head. The grid has one block per item; a running CTA takes over blocks that have not started
 // (clc_request), so items of uneven cost balance over the SMs without a counter in memory that two launches
@@ -214,7 +214,7 @@ __device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool w
 //              the softmax warps as 16-bit pairs over S_X, is the A operand of O_X += P_X V_t -> TMEM
 //              [256X + 128, +D). Order at key tile t: PV_A(t) S_A(t+1) PV_B(t) S_B(t+1), so the tensor core
 //              works on one query tile while the other's softmax runs;
-//   warps 2-9  softmax, one query row per thread (2-5 tile A, 6-9 tile B).
+//   warps 4-11 softmax, one query row per thread (4-7 tile A, 8-11 tile B).
 // S_X(t+1) is issued after PV_X(t) and the MMAs of a CTA complete in order, so a softmax warp that sees S_X(t+1) may
 // overwrite P_X and rescale O_X. P is at most 2^8 (the running maximum is only replaced when it grows by more
 // than that) and is rounded to 16 bits for the product (half a step, relative); the row sum l adds the
@@ -244,7 +244,21 @@ __device__ __forceinline__ void load_tile(const CUtensorMap* m, bool swap, uint6
     tma_load_3d(m, bar, dst + c * atom_bytes, 64 * c, swap ? row : head, swap ? head : row);
 }
 
+// The blocks of these kernels are three warpgroups, launched with 168 registers a thread (64512 of an SM's 65536):
+// the first one, which loads and issues, gives most of its share up and the two that hold a score row per
+// thread take it: 128 x (104 + 200 + 200) = 64512.
+__device__ __forceinline__ void few_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); }
+__device__ __forceinline__ void many_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); }
+
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Shared-memory descriptors of a tile whose rows run along the product's free index (K-major: a step of 16 along D
+// is 32 bytes inside an atom) or along its summed one (MN-major: 16 rows are 2048 bytes; atom: bytes of an atom
+// column). The address field counts 16 bytes and has no carry into the next, so steps are added to it.
+__device__ __forceinline__ uint64_t k_major(const void* tile) { return umma_desc_sw128(smem_u32(tile), 16, 1024); }
+__device__ __forceinline__ uint64_t mn_major(const void* tile, uint32_t atom) {
+  return umma_desc_sw128(smem_u32(tile), atom, 1024);
+}
 
 struct FwdItem {
   int h[2], q0[2];  // head and first row of the query tiles A and B
@@ -283,7 +297,7 @@ __device__ __forceinline__ void item_keys(FwdItem& I, const PackedParams& p) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(320, 1) fwd_tc_kernel(const __grid_constant__ FwdMaps maps,
+__global__ void __launch_bounds__(384, 1) fwd_tc_kernel(const __grid_constant__ FwdMaps maps,
                                                         const __grid_constant__ PackedParams p, int* status) {
   using C = FwdCfg<D>;
   constexpr int kAtoms = D / 64;
@@ -354,6 +368,7 @@ __global__ void __launch_bounds__(320, 1) fwd_tc_kernel(const __grid_constant__ 
   };
 
   if (warp == 0) {
+    few_registers();
     if (elect_one()) {
       tma_prefetch_desc(&maps.q);
       tma_prefetch_desc(&maps.k);
@@ -431,6 +446,7 @@ __global__ void __launch_bounds__(320, 1) fwd_tc_kernel(const __grid_constant__ 
       }
     }
   } else if (warp == 1) {
+    few_registers();
     if (elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc_16<T>(BT, BT, false, false);
       constexpr uint32_t idesc_o = umma_idesc_16<T>(BT, D, false, true);
@@ -453,12 +469,11 @@ __global__ void __launch_bounds__(320, 1) fwd_tc_kernel(const __grid_constant__ 
           const int g = kbase + t - t0, st = g % C::kK;
           if (!wait(&k_full[st], g / C::kK)) return false;
           tc_fence_after();
-          const uint32_t q_addr = smem_u32(smem + C::oQ + x * C::kTile), k_addr = smem_u32(smem + C::oK + st * C::kTile);
+          const uint64_t q_desc = k_major(smem + C::oQ + x * C::kTile), k_desc = k_major(smem + C::oK + st * C::kTile);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 32;
-            umma_bf16_ss(tmem + x * 256, umma_desc_sw128(q_addr + off, 16, 1024), umma_desc_sw128(k_addr + off, 16, 1024),
-                         idesc_s, kk > 0 ? 1u : 0u);
+            const uint32_t off = ((kk >> 2) * kAtom + (kk & 3) * 32) >> 4;
+            umma_bf16_ss(tmem + x * 256, q_desc + off, k_desc + off, idesc_s, kk > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[x]);
           if (x == 1 || !I.uses(1, t)) umma_commit(&k_empty[st]);  // the tile's last reader
@@ -472,11 +487,11 @@ __global__ void __launch_bounds__(320, 1) fwd_tc_kernel(const __grid_constant__ 
           if (!wait(&p_full[x], pc[x]) || !wait(&v_full[st], g / C::kV)) return false;
           ++pc[x];
           tc_fence_after();
-          const uint32_t v_addr = smem_u32(smem + C::oV + st * C::kTile);
+          const uint64_t v_desc = mn_major(smem + C::oV + st * C::kTile, kAtom);
 #pragma unroll
           for (int kk = 0; kk < BT / 16; ++kk)
-            umma_bf16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, umma_desc_sw128(v_addr + kk * 2048, kAtom, 1024),
-                         idesc_o, (t > I.lo[x] || kk > 0) ? 1u : 0u);
+            umma_bf16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, v_desc + kk * (2048 >> 4), idesc_o,
+                         (t > I.lo[x] || kk > 0) ? 1u : 0u);
           if (x == 1 || !I.uses(1, t)) umma_commit(&v_empty[st]);
           if (t == I.hi[x] - 1) {
             umma_commit(&o_done[x]);
@@ -497,8 +512,11 @@ __global__ void __launch_bounds__(320, 1) fwd_tc_kernel(const __grid_constant__ 
       umma_commit(drain);
       mbar_wait(drain, 0, kDrainNs, nullptr);
     }
+  } else if (warp < 4) {
+    few_registers();
   } else {
-    const int x = (warp - 2) >> 2, wq = warp & 3, lane = lane_id();
+    many_registers();
+    const int x = (warp - 4) >> 2, wq = warp & 3, lane = lane_id();
     const int r = wq * 32 + lane;  // row of the tile = TMEM lane
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16) + x * 256;
     int sc = 0, oc = 0;  // score blocks consumed and items finished by this query tile
@@ -536,70 +554,74 @@ __global__ void __launch_bounds__(320, 1) fwd_tc_kernel(const __grid_constant__ 
         }
         tc_fence_after();
         const int k0 = t * BT;
-        uint32_t sr[4][32];  // this row's scores before scaling
+        const bool all = __all_sync(0xffffffffu, key.x <= k0 && key.y >= k0 + BT);  // no key of the tile is hidden
+        // P = exp2(S scale - m) with the maximum so far: one pass, in which the tile's own maximum is found beside the
+        // exponentials. Only where that exceeds the old one by more than 2^8 (and in the first tile) are the
+        // scores read again and the exponentials taken anew. P replaces S in TMEM once it stands.
+        uint32_t pk[64];
+        float mx, add;
+        auto pass = [&](bool first) {
+          uint32_t sr[4][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(lane_base + c * 32, sr[c]);
-        tmem_ld_wait();
-        float mx = -INFINITY;
-        if (__all_sync(0xffffffffu, key.x <= k0 && key.y >= k0 + BT)) {
-          // every key of the tile is visible to the warp's rows
+          for (int c = 0; c < 4; ++c) tmem_ld32(lane_base + c * 32, sr[c]);
+          tmem_ld_wait();
+          if (!all) {
 #pragma unroll
-          for (int e = 0; e < BT; ++e) mx = fmaxf(mx, __uint_as_float(sr[e >> 5][e & 31]));
-        } else {
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t vis = range_mask32(key.x - k0 - 32 * c, key.y - k0 - 32 * c);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t vis = range_mask32(key.x - k0 - 32 * c, key.y - k0 - 32 * c);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float s = ((vis >> e) & 1u) ? __uint_as_float(sr[c][e]) : -INFINITY;
-              sr[c][e] = __float_as_uint(s);
-              mx = fmaxf(mx, s);
+              for (int e = 0; e < 32; ++e) sr[c][e] = ((vis >> e) & 1u) ? sr[c][e] : 0xff800000u;
             }
           }
-        }
-        mx *= p.scale_log2;
-        // The rescale is decided per row, but tcgen05.ld/st are warp-collective: the warp rescales together
-        // when any of its rows needs it, the others by 1.
-        float alpha = 1.f;
-        bool mine = false;
-        if (t == t_lo) {
-          m_ref = mx;
-        } else if (mx > m_ref + 8.f) {
-          mine = true;
-          alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
-          l *= alpha;
-          m_ref = mx;
-        }
-        if (__any_sync(0xffffffffu, mine)) {
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t v[32];
-            tmem_ld32(lane_base + 128 + c * 32, v);
-            tmem_ld_wait();
+          float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (first) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-            tmem_st32(lane_base + 128 + c * 32, v);
+            for (int e = 0; e < BT; ++e) part[e & 3] = fmaxf(part[e & 3], __uint_as_float(sr[e >> 5][e & 31]));
+            m_ref = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * p.scale_log2;
           }
-        }
-        const float mref = m_ref == -INFINITY ? 0.f : m_ref;
-        const uint64_t sc2 = f32x2(p.scale_log2, p.scale_log2), nm2 = f32x2(-mref, -mref);
-        uint64_t l2 = f32x2(0.f, 0.f);
+          const float mref = m_ref == -INFINITY ? 0.f : m_ref;
+          const uint64_t sc2 = f32x2(p.scale_log2, p.scale_log2), nm2 = f32x2(-mref, -mref);
+          uint64_t l2[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int e = 0; e < 64; e += 2) {
-            const int a = c * 64 + e;
-            const float2 y = f32x2_split(fma_f32x2(
-                f32x2(__uint_as_float(sr[a >> 5][a & 31]), __uint_as_float(sr[a >> 5][(a + 1) & 31])), sc2, nm2));
+          for (int e = 0; e < BT; e += 2) {
+            const float s0 = __uint_as_float(sr[e >> 5][e & 31]), s1 = __uint_as_float(sr[e >> 5][(e + 1) & 31]);
+            part[(e >> 1) & 3] = fmaxf(fmaxf(part[(e >> 1) & 3], s0), s1);
+            const float2 y = f32x2_split(fma_f32x2(f32x2(s0, s1), sc2, nm2));
             const float p0 = exp2f(y.x), p1 = exp2f(y.y);
-            l2 = add_f32x2(l2, f32x2(p0, p1));
+            l2[(e >> 1) & 1] = add_f32x2(l2[(e >> 1) & 1], f32x2(p0, p1));
             pk[e / 2] = Half16<T>::pack(p0, p1);
           }
-          tmem_st32(lane_base + c * 32, pk);
+          mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * p.scale_log2;
+          const float2 ls = f32x2_split(add_f32x2(l2[0], l2[1]));
+          add = ls.x + ls.y;
+        };
+        pass(t == t_lo);
+        // The rescale is decided per row, but tcgen05.ld/st are warp-collective: the warp rescales together
+        // when any of its rows needs it, the others by 1.
+        if (t > t_lo) {
+          const bool mine = mx > m_ref + 8.f;
+          if (__any_sync(0xffffffffu, mine)) {
+            float alpha = 1.f;
+            if (mine) {
+              alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
+              l *= alpha;
+              m_ref = mx;
+            }
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t v[32];
+              tmem_ld32(lane_base + 128 + c * 32, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+              tmem_st32(lane_base + 128 + c * 32, v);
+            }
+            pass(false);
+          }
         }
-        const float2 ls = f32x2_split(l2);
-        l += ls.x + ls.y;
+        l += add;
+        tmem_st32(lane_base, *reinterpret_cast<const uint32_t(*)[32]>(pk));
+        tmem_st32(lane_base + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
         if (t == t_lo && clears) {
           if (!wait(&v_full[vfirst % C::kV], vfirst / C::kV)) *abort_flag = 1;
           uint4* row = reinterpret_cast<uint4*>(smem + C::oV + vfirst % C::kV * C::kTile + r * 128);
@@ -677,10 +699,11 @@ __global__ void __launch_bounds__(320, 1) fwd_tc_kernel(const __grid_constant__ 
 // ---------------------------------------------------------------------------------------- backward, tcgen05
 // Two kernels, so that no sum is shared between blocks and the results do not depend on the schedule: dQ (one block
 // per 128 query rows and head) and dK/dV (one block per 128 key rows and kv head). Both recompute the scores,
-// 64 keys or queries at a time, 320 threads: warp 0 loads (TMA), warp 1 issues the MMAs, warps 2-9 turn scores
-// into P and dS, one tile row per thread, warps w and w + 4 sharing the rows of TMEM lane group w % 4 and
-// splitting the block's 64 columns. P and dS are rounded to 16 bits for their products (half a step, relative to
-// each entry); everything else is fp32. A warp writes its 16-bit results over the scores that it has itself read.
+// 64 keys or queries at a time, 384 threads: warp 0 loads (TMA), warp 1 issues the MMAs, warps 4-7 and 8-11 turn
+// scores into P and dS, one tile row per thread, the two groups taking the blocks in turn: while one group
+// loads, computes and stores, the other's block goes through the tensor core. P and dS are rounded to 16 bits
+// for their products (half a step, relative to each entry); everything else is fp32. They are written over the
+// scores that they came from.
 constexpr int BB = 64;  // keys (dQ) or queries (dK/dV) of a block
 constexpr int kAtom64 = BB * 128;
 
@@ -719,8 +742,7 @@ __device__ __forceinline__ bool store_cols(uint32_t taddr, float f, T* dst, bool
   return odd != 0.f;
 }
 
-// dQ. TMEM: two score sets (set s: S at [128s, +64), dP at [128s + 64, +64)), so that block j + 1's scores are
-// computed while block j is turned into dS; dQ at [256, +D); the block's Q and dO rows as 16-bit pairs at [384, +D/2)
+// dQ. TMEM: two score sets (set s, for the blocks of group s: S at [128s, +64), dP at [128s + 64, +64)); dQ at [256, +D); the block's Q and dO rows as 16-bit pairs at [384, +D/2)
 // and [448, +D/2): the S and dP products read only K and V from shared memory. The kernel also computes
 // delta = rowsum(dO o O) and leaves (lse, delta) of each row for the dK/dV kernel.
 template <int D>
@@ -739,7 +761,7 @@ struct DqMaps {
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(320, 1) dq_tc_kernel(const __grid_constant__ DqMaps maps,
+__global__ void __launch_bounds__(384, 1) dq_tc_kernel(const __grid_constant__ DqMaps maps,
                                                        const __grid_constant__ PackedParams p, int* status) {
   using C = DqCfg<D>;
   constexpr int kAtoms = D / 64;
@@ -749,7 +771,7 @@ __global__ void __launch_bounds__(320, 1) dq_tc_kernel(const __grid_constant__ D
   uint64_t* q_full = bars + 0;
   uint64_t* done = bars + 1;
   uint64_t* s_full = bars + 2;  // [2]
-  uint64_t* p_full = bars + 4;  // [2], by block parity: a warp group one block ahead arrives on the other barrier
+  uint64_t* p_full = bars + 4;  // [2]
   uint64_t* kv_full = bars + 6;
   uint64_t* kv_empty = kv_full + C::kStages;
   static_assert(6 + 2 * C::kStages <= 28, "barrier region");
@@ -769,7 +791,7 @@ __global__ void __launch_bounds__(320, 1) dq_tc_kernel(const __grid_constant__ D
     mbar_init(done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 256);
+      mbar_init(&p_full[i], 128);
     }
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -790,6 +812,7 @@ __global__ void __launch_bounds__(320, 1) dq_tc_kernel(const __grid_constant__ D
   auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, kBudgetNs, abort_flag, status); };
 
   if (warp == 0) {
+    few_registers();
     if (elect_one()) {
       int j = 0;
       bool ok = true;
@@ -811,6 +834,7 @@ __global__ void __launch_bounds__(320, 1) dq_tc_kernel(const __grid_constant__ D
       }
     }
   } else if (warp == 1) {
+    few_registers();
     if (elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc_16<T>(BT, BB, false, false);
       constexpr uint32_t idesc_q = umma_idesc_16<T>(BT, D, false, true);
@@ -819,41 +843,42 @@ __global__ void __launch_bounds__(320, 1) dq_tc_kernel(const __grid_constant__ D
         const int st = j % C::kStages, set = j & 1;
         if (!wait(&kv_full[st], j / C::kStages)) return false;
         tc_fence_after();
-        const uint32_t k_addr = smem_u32(smem + C::oK + st * C::kTile), v_addr = smem_u32(smem + C::oV + st * C::kTile);
+        const uint64_t k_desc = k_major(smem + C::oK + st * C::kTile), v_desc = k_major(smem + C::oV + st * C::kTile);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kAtom64 + (kk & 3) * 32;
-          umma_bf16_ts(tmem + set * 128, tmem + 384 + kk * 8, umma_desc_sw128(k_addr + off, 16, 1024), idesc_s,
-                       kk > 0 ? 1u : 0u);
-          umma_bf16_ts(tmem + set * 128 + 64, tmem + 448 + kk * 8, umma_desc_sw128(v_addr + off, 16, 1024), idesc_s,
-                       kk > 0 ? 1u : 0u);
+          const uint32_t off = ((kk >> 2) * kAtom64 + (kk & 3) * 32) >> 4;
+          umma_bf16_ts(tmem + set * 128, tmem + 384 + kk * 8, k_desc + off, idesc_s, kk > 0 ? 1u : 0u);
+          umma_bf16_ts(tmem + set * 128 + 64, tmem + 448 + kk * 8, v_desc + off, idesc_s, kk > 0 ? 1u : 0u);
         }
         umma_commit(&s_full[set]);
         return true;
       };
       if (ok) ok = issue_s(0);
+      if (ok && nb > 1) ok = issue_s(1);
       for (int j = 0; j < nb && ok; ++j) {
-        if (j + 1 < nb && !issue_s(j + 1)) ok = false;
-        if (!ok || !wait(&p_full[j & 1], j >> 1)) {
+        if (!wait(&p_full[j & 1], j >> 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
         const int st = j % C::kStages;
-        const uint32_t k_addr = smem_u32(smem + C::oK + st * C::kTile);
-        // dS of keys 32h .. 32h + 31 sits at columns 128 set + 32h .. + 15
+        const uint64_t k_desc = mn_major(smem + C::oK + st * C::kTile, kAtom64);
 #pragma unroll
-        for (int kk = 0; kk < BB / 16; ++kk)
-          umma_bf16_ts(tmem + 256, tmem + (j & 1) * 128 + (kk >> 1) * 32 + (kk & 1) * 8,
-                       umma_desc_sw128(k_addr + kk * 2048, kAtom64, 1024), idesc_q, (j > 0 || kk > 0) ? 1u : 0u);
+        for (int kk = 0; kk < BB / 16; ++kk)  // dS as 16-bit pairs at the first 32 columns of its set
+          umma_bf16_ts(tmem + 256, tmem + (j & 1) * 128 + kk * 8, k_desc + kk * (2048 >> 4), idesc_q,
+                       (j > 0 || kk > 0) ? 1u : 0u);
         umma_commit(&kv_empty[st]);
+        if (j + 2 < nb) ok = issue_s(j + 2);  // into the set that this product has read
       }
       if (!ok) fail(kErrTimeoutMma);
       umma_commit(done);
       mbar_wait(done, 0, kBudgetNs, nullptr);
     }
+  } else if (warp < 4) {
+    few_registers();
   } else {
-    const int wq = warp & 3, lane = lane_id(), half = (warp - 2) >> 2;
+    many_registers();
+    const int wq = warp & 3, lane = lane_id(), half = (warp - 4) >> 2;
     const int r = wq * 32 + lane, i = q0 + r, ic = min(i, p.N - 1);
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16);
     const int2 key = i < p.N ? keys_of(p, i) : make_int2(0, 0);
@@ -902,58 +927,65 @@ __global__ void __launch_bounds__(320, 1) dq_tc_kernel(const __grid_constant__ D
       asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps
       stat = real ? make_float2(p.lse[(int64_t)h * p.N + i] * kLog2e, sums[r] + sums[128 + r])
                   : make_float2(INFINITY, 0.f);
-      if (half == 0) p.stat[(int64_t)h * p.Np + i] = stat;
+      if (half == 0) p.stat[(int64_t)h * p.Np + i] = make_float2(-stat.x, -stat.y);
     }
     const int z = __ldg(p.start + q0);  // keys before it are foreign to every row of the tile: all in block kb_lo
     bool ok = true;
-    for (int j = 0; j < nb; ++j) {
-      const int set = j & 1;
-      if (!mbar_wait_warp(&s_full[set], (j >> 1) & 1, kBudgetNs, abort_flag, status)) {
+    const uint32_t set_base = lane_base + half * 128;
+    for (int j = half; j < nb; j += 2) {
+      if (!mbar_wait_warp(&s_full[half], (j >> 1) & 1, kBudgetNs, abort_flag, status)) {
         fail(kErrTimeoutEpilogue);
         ok = false;
         break;
       }
       tc_fence_after();
-      const int k0 = (kb_lo + j) * BB + half * 32;
-      uint32_t sv[32], dv[32], pk[16];
-      tmem_ld32(lane_base + set * 128 + half * 32, sv);
-      tmem_ld32(lane_base + set * 128 + 64 + half * 32, dv);
-      tmem_ld_wait();
+      const int k0 = (kb_lo + j) * BB;
+      uint32_t pk[32];
       // dS = P (dP - delta), 0 where the row does not see the key
-      auto body = [&](auto masked) {
+      uint32_t svs[2][32], dvs[2][32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        tmem_ld32(set_base + c * 32, svs[c]);
+        tmem_ld32(set_base + 64 + c * 32, dvs[c]);
+      }
+      tmem_ld_wait();
+      auto body = [&](int c, auto masked) {
         constexpr bool kMasked = decltype(masked)::value;
+        const uint32_t(&sv)[32] = svs[c];
+        const uint32_t(&dv)[32] = dvs[c];
         uint32_t vis = 0xffffffffu;
-        if constexpr (kMasked) vis = range_mask32(key.x - k0, key.y - k0);
-        const uint64_t dl2 = f32x2(stat.y, stat.y);
+        if constexpr (kMasked) vis = range_mask32(key.x - k0 - 32 * c, key.y - k0 - 32 * c);
+        const uint64_t dl2 = f32x2(stat.y, stat.y), sc2 = f32x2(p.scale_log2, p.scale_log2), nl2 = f32x2(-stat.x, -stat.x);
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float p0 = exp2f(fmaf(__uint_as_float(sv[e]), p.scale_log2, -stat.x));
-          const float p1 = exp2f(fmaf(__uint_as_float(sv[e + 1]), p.scale_log2, -stat.x));
-          float2 g = f32x2_split(
-              mul_f32x2(f32x2(p0, p1), sub_f32x2(f32x2(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), dl2)));
+          const float2 y = f32x2_split(fma_f32x2(f32x2(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), sc2, nl2));
+          float2 g = f32x2_split(mul_f32x2(f32x2(exp2f(y.x), exp2f(y.y)),
+                                           sub_f32x2(f32x2(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), dl2)));
           if constexpr (kMasked) {
             g.x = ((vis >> e) & 1u) ? g.x : 0.f;
             g.y = ((vis >> (e + 1)) & 1u) ? g.y : 0.f;
           }
-          pk[e / 2] = Half16<T>::pack(g.x, g.y);
+          pk[c * 16 + e / 2] = Half16<T>::pack(g.x, g.y);
         }
       };
-      if (__all_sync(0xffffffffu, key.x <= k0 && key.y >= k0 + 32)) {
-        body(std::false_type{});
+      if (__all_sync(0xffffffffu, key.x <= k0 && key.y >= k0 + BB)) {
+        body(0, std::false_type{});
+        body(1, std::false_type{});
       } else {
-        body(std::true_type{});
+        body(0, std::true_type{});
+        body(1, std::true_type{});
       }
-      if (j == 0 && half == 0 && r < BB && kb_lo * BB + r < z) {
+      if (j == 0 && r < BB && kb_lo * BB + r < z) {
         uint4* row = reinterpret_cast<uint4*>(smem + C::oK + r * 128);
 #pragma unroll 1
         for (int c = 0; c < D / 64 * 8; ++c) row[(c >> 3) * (kAtom64 / 16) + (c & 7)] = make_uint4(0, 0, 0, 0);
         fence_async_smem();
       }
       __syncwarp();
-      tmem_st16(lane_base + set * 128 + half * 32, pk);
+      tmem_st32(set_base, pk);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[j & 1]);
+      mbar_arrive(&p_full[half]);
     }
     if (ok && mbar_wait_warp(done, 0, kBudgetNs, abort_flag, status)) {
       tc_fence_after();
@@ -984,7 +1016,7 @@ __global__ void __launch_bounds__(320, 1) dq_tc_kernel(const __grid_constant__ D
   }
 }
 
-// dK and dV. TMEM: two score sets (set s: S^T at [128s, +64), dP^T at [128s + 64, +64)), dV at [256, +D), dK at
+// dK and dV. TMEM: two score sets (set s, for the blocks of group s: S^T at [128s, +64), dP^T at [128s + 64, +64)), dV at [256, +D), dK at
 // [384, +D). K and V stay in shared memory as the A operands of S^T and dP^T; blocks of 64 queries (Q, dO, their
 // lse and delta) go through a ring, head after head of the kv head's group.
 template <int D>
@@ -1003,7 +1035,7 @@ struct DkvMaps {
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(320, 1) dkv_tc_kernel(const __grid_constant__ DkvMaps maps,
+__global__ void __launch_bounds__(384, 1) dkv_tc_kernel(const __grid_constant__ DkvMaps maps,
                                                         const __grid_constant__ PackedParams p, int* status) {
   using C = DkvCfg<D>;
   constexpr int kAtoms = D / 64;
@@ -1013,7 +1045,7 @@ __global__ void __launch_bounds__(320, 1) dkv_tc_kernel(const __grid_constant__ 
   uint64_t* kv_full = bars + 0;
   uint64_t* done = bars + 1;
   uint64_t* s_full = bars + 2;  // [2]
-  uint64_t* p_full = bars + 4;  // [2], by iteration parity
+  uint64_t* p_full = bars + 4;  // [2]
   uint64_t* qd_full = bars + 6;
   uint64_t* qd_empty = qd_full + C::kStages;
   static_assert(6 + 2 * C::kStages <= 28, "barrier region");
@@ -1033,7 +1065,7 @@ __global__ void __launch_bounds__(320, 1) dkv_tc_kernel(const __grid_constant__ 
     mbar_init(done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 256);
+      mbar_init(&p_full[i], 128);
     }
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&qd_full[i], 1);
@@ -1054,6 +1086,7 @@ __global__ void __launch_bounds__(320, 1) dkv_tc_kernel(const __grid_constant__ 
   auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, kBudgetNs, abort_flag, status); };
 
   if (warp == 0) {
+    few_registers();
     if (elect_one()) {
       mbar_arrive_expect_tx(kv_full, 2 * C::kTile);
       load_tile(&maps.k, maps.swap_kv & 1, kv_full, smem + C::oK, kvh, k0, kAtoms, kAtom);
@@ -1080,53 +1113,57 @@ __global__ void __launch_bounds__(320, 1) dkv_tc_kernel(const __grid_constant__ 
       }
     }
   } else if (warp == 1) {
+    few_registers();
     if (elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc_16<T>(BT, BB, false, false);
       constexpr uint32_t idesc_g = umma_idesc_16<T>(BT, D, false, true);
-      const uint32_t k_addr = smem_u32(smem + C::oK), v_addr = smem_u32(smem + C::oV);
+      const uint64_t k_desc = k_major(smem + C::oK), v_desc = k_major(smem + C::oV);
       bool ok = wait(kv_full, 0);
       auto issue_s = [&](int it) -> bool {
         const int st = it % C::kStages, set = it & 1;
         if (!wait(&qd_full[st], it / C::kStages)) return false;
         tc_fence_after();
-        const uint32_t q_addr = smem_u32(smem + C::oQ + st * C::kBlock), d_addr = smem_u32(smem + C::oD + st * C::kBlock);
+        const uint64_t q_desc = k_major(smem + C::oQ + st * C::kBlock), d_desc = k_major(smem + C::oD + st * C::kBlock);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t offa = (kk >> 2) * kAtom + (kk & 3) * 32, offb = (kk >> 2) * kAtom64 + (kk & 3) * 32;
-          umma_bf16_ss(tmem + set * 128, umma_desc_sw128(k_addr + offa, 16, 1024),
-                       umma_desc_sw128(q_addr + offb, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
-          umma_bf16_ss(tmem + set * 128 + 64, umma_desc_sw128(v_addr + offa, 16, 1024),
-                       umma_desc_sw128(d_addr + offb, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+          const uint32_t offa = ((kk >> 2) * kAtom + (kk & 3) * 32) >> 4, offb = ((kk >> 2) * kAtom64 + (kk & 3) * 32) >> 4;
+          umma_bf16_ss(tmem + set * 128, k_desc + offa, q_desc + offb, idesc_s, kk > 0 ? 1u : 0u);
+          umma_bf16_ss(tmem + set * 128 + 64, v_desc + offa, d_desc + offb, idesc_s, kk > 0 ? 1u : 0u);
         }
         umma_commit(&s_full[set]);
         return true;
       };
       if (ok) ok = issue_s(0);
+      if (ok && iters > 1) ok = issue_s(1);
       for (int it = 0; it < iters && ok; ++it) {
-        if (it + 1 < iters && !issue_s(it + 1)) ok = false;
-        if (!ok || !wait(&p_full[it & 1], it >> 1)) {
+        if (!wait(&p_full[it & 1], it >> 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
         const int st = it % C::kStages, set = it & 1;
-        const uint32_t q_addr = smem_u32(smem + C::oQ + st * C::kBlock), d_addr = smem_u32(smem + C::oD + st * C::kBlock);
-        // P^T and dS^T of queries 32h .. 32h + 31 sit at columns 32h .. + 15 of S^T and dP^T
+        const uint64_t q_desc = mn_major(smem + C::oQ + st * C::kBlock, kAtom64);
+        const uint64_t d_desc = mn_major(smem + C::oD + st * C::kBlock, kAtom64);
+        // P^T and dS^T as 16-bit pairs at the first 32 columns of S^T and dP^T
 #pragma unroll
         for (int kk = 0; kk < BB / 16; ++kk) {
           const uint32_t acc = (it > 0 || kk > 0) ? 1u : 0u;
-          const uint32_t col = tmem + set * 128 + (kk >> 1) * 32 + (kk & 1) * 8;
-          umma_bf16_ts(tmem + 256, col, umma_desc_sw128(d_addr + kk * 2048, kAtom64, 1024), idesc_g, acc);
-          umma_bf16_ts(tmem + 384, col + 64, umma_desc_sw128(q_addr + kk * 2048, kAtom64, 1024), idesc_g, acc);
+          const uint32_t col = tmem + set * 128 + kk * 8;
+          umma_bf16_ts(tmem + 256, col, d_desc + kk * (2048 >> 4), idesc_g, acc);
+          umma_bf16_ts(tmem + 384, col + 64, q_desc + kk * (2048 >> 4), idesc_g, acc);
         }
         umma_commit(&qd_empty[st]);
+        if (it + 2 < iters) ok = issue_s(it + 2);  // into the set that these products have read
       }
       if (!ok) fail(kErrTimeoutMma);
       umma_commit(done);
       mbar_wait(done, 0, kBudgetNs, nullptr);
     }
+  } else if (warp < 4) {
+    few_registers();
   } else {
-    const int wq = warp & 3, lane = lane_id(), half = (warp - 2) >> 2;
+    many_registers();
+    const int wq = warp & 3, lane = lane_id(), half = (warp - 4) >> 2;
     const int r = wq * 32 + lane, j = k0 + r;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16);
     // the queries that see this key row (none for a row of no sequence)
@@ -1134,31 +1171,40 @@ __global__ void __launch_bounds__(320, 1) dkv_tc_kernel(const __grid_constant__ 
     const int q_hi = real ? queries_of(p, j) : 0;
     const int z = __ldg(p.end + k_last);  // queries from here on are foreign to every key of the tile: all in block qb_hi
     bool ok = true;
-    for (int it = 0; it < iters; ++it) {
-      const int set = it & 1, st = it % C::kStages;
-      if (!mbar_wait_warp(&s_full[set], (it >> 1) & 1, kBudgetNs, abort_flag, status)) {
+    const uint32_t set_base = lane_base + half * 128;
+    int qb = half % nq;  // the iteration's query block, counted from qb_lo
+    for (int it = half; it < iters; it += 2) {
+      const int st = it % C::kStages;
+      if (!mbar_wait_warp(&s_full[half], (it >> 1) & 1, kBudgetNs, abort_flag, status)) {
         fail(kErrTimeoutEpilogue);
         ok = false;
         break;
       }
       tc_fence_after();
-      const int q0 = (qb_lo + it % nq) * BB + half * 32;
-      const float4* ls = reinterpret_cast<const float4*>(stat + st * BB + half * 32);
-      uint32_t sv[32], dv[32], pp[16], ss[16];
-      tmem_ld32(lane_base + set * 128 + half * 32, sv);
-      tmem_ld32(lane_base + set * 128 + 64 + half * 32, dv);
+      const int q0 = (qb_lo + qb) * BB;
+      uint32_t pp[32], ss[32], svs[2][32], dvs[2][32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        tmem_ld32(set_base + c * 32, svs[c]);
+        tmem_ld32(set_base + 64 + c * 32, dvs[c]);
+      }
       tmem_ld_wait();
-      auto body = [&](auto masked) {
+      auto body = [&](int c, auto masked) {
         constexpr bool kMasked = decltype(masked)::value;
+        const float4* ls = reinterpret_cast<const float4*>(stat + st * BB + c * 32);
+        const uint32_t(&sv)[32] = svs[c];
+        const uint32_t(&dv)[32] = dvs[c];
         uint32_t vis = 0xffffffffu;
-        if constexpr (kMasked) vis = range_mask32(real ? j - q0 : 32, q_hi - q0);
+        if constexpr (kMasked) vis = range_mask32(real ? j - q0 - 32 * c : 32, q_hi - q0 - 32 * c);
+        const uint64_t sc2 = f32x2(p.scale_log2, p.scale_log2);
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float4 a = ls[e / 2];  // (lse, delta) of two queries
-          float p0 = exp2f(fmaf(__uint_as_float(sv[e]), p.scale_log2, -a.x));
-          float p1 = exp2f(fmaf(__uint_as_float(sv[e + 1]), p.scale_log2, -a.z));
+          const float4 a = ls[e / 2];  // (-lse, -delta) of two queries
+          const float2 y = f32x2_split(fma_f32x2(f32x2(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), sc2,
+                                                 f32x2(a.x, a.z)));
+          float p0 = exp2f(y.x), p1 = exp2f(y.y);
           float2 g = f32x2_split(mul_f32x2(
-              f32x2(p0, p1), sub_f32x2(f32x2(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), f32x2(a.y, a.w))));
+              f32x2(p0, p1), add_f32x2(f32x2(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), f32x2(a.y, a.w))));
           if constexpr (kMasked) {
             const bool v0 = (vis >> e) & 1u, v1 = (vis >> (e + 1)) & 1u;
             p0 = v0 ? p0 : 0.f;
@@ -1166,16 +1212,18 @@ __global__ void __launch_bounds__(320, 1) dkv_tc_kernel(const __grid_constant__ 
             g.x = v0 ? g.x : 0.f;
             g.y = v1 ? g.y : 0.f;
           }
-          pp[e / 2] = Half16<T>::pack(p0, p1);
-          ss[e / 2] = Half16<T>::pack(g.x, g.y);
+          pp[c * 16 + e / 2] = Half16<T>::pack(p0, p1);
+          ss[c * 16 + e / 2] = Half16<T>::pack(g.x, g.y);
         }
       };
-      if (__all_sync(0xffffffffu, real && j <= q0 && q_hi >= q0 + 32)) {
-        body(std::false_type{});
+      if (__all_sync(0xffffffffu, real && j <= q0 && q_hi >= q0 + BB)) {
+        body(0, std::false_type{});
+        body(1, std::false_type{});
       } else {
-        body(std::true_type{});
+        body(0, std::true_type{});
+        body(1, std::true_type{});
       }
-      if (it % nq == nq - 1 && half == 0 && r < BB && qb_hi * BB + r >= z) {
+      if (qb == nq - 1 && r < BB && qb_hi * BB + r >= z) {
         uint4* row = reinterpret_cast<uint4*>(smem + C::oQ + st * C::kBlock + r * 128);
         uint4* dow = reinterpret_cast<uint4*>(smem + C::oD + st * C::kBlock + r * 128);
 #pragma unroll 1
@@ -1184,11 +1232,13 @@ __global__ void __launch_bounds__(320, 1) dkv_tc_kernel(const __grid_constant__ 
         fence_async_smem();
       }
       __syncwarp();
-      tmem_st16(lane_base + set * 128 + half * 32, pp);
-      tmem_st16(lane_base + set * 128 + 64 + half * 32, ss);
+      tmem_st32(set_base, pp);
+      tmem_st32(set_base + 64, ss);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[it & 1]);
+      mbar_arrive(&p_full[half]);
+      qb += 2;
+      while (qb >= nq) qb -= nq;
     }
     if (ok && mbar_wait_warp(done, 0, kBudgetNs, abort_flag, status)) {
       tc_fence_after();
@@ -1367,7 +1417,7 @@ std::tuple<torch::Tensor, torch::Tensor> packed_attn_fwd(const torch::Tensor& q,
     const int64_t tiles = (p.N + BT - 1) / BT;
     const int64_t items = p.H / p.KV % 2 == 0 ? tiles * (p.H / 2) : (tiles + 1) / 2 * p.H;
     TORCH_CHECK_VALUE(items < (int64_t(1) << 31), what, ": too many rows or heads");
-    fwd_tc_kernel<decltype(t), D><<<(unsigned)items, 320, C::kSmem, st>>>(maps, p, status_ptr(q.device().index()));
+    fwd_tc_kernel<decltype(t), D><<<(unsigned)items, 384, C::kSmem, st>>>(maps, p, status_ptr(q.device().index()));
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {out, lse};
@@ -1427,9 +1477,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
     const int64_t tiles = p.Np / BT;
     TORCH_CHECK_VALUE(tiles * H < (int64_t(1) << 31), what, ": too many rows or heads");
     int* status = status_ptr(q.device().index());
-    dq_tc_kernel<T, D><<<(unsigned)(tiles * H), 320, DqCfg<D>::kSmem, st>>>(a, p, status);
+    dq_tc_kernel<T, D><<<(unsigned)(tiles * H), 384, DqCfg<D>::kSmem, st>>>(a, p, status);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
-    dkv_tc_kernel<T, D><<<(unsigned)(tiles * KV), 320, DkvCfg<D>::kSmem, st>>>(b, p, status);
+    dkv_tc_kernel<T, D><<<(unsigned)(tiles * KV), 384, DkvCfg<D>::kSmem, st>>>(b, p, status);
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {dq, dk, dv};
