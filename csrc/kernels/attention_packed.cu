@@ -208,34 +208,58 @@ __device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool w
 // tiles of one head. The grid has one block per item; a running CTA takes over blocks that have not started
 // (clc_request), so items of uneven cost balance over the SMs without a counter in memory that two launches
 // would share. Items go from the last rows to the first: in a long sequence the late rows cost most.
-//   warp 0     takes items, hands them to the other warps through a two-slot ring, and issues the TMA loads: the
-//              item's two Q tiles, then K and V tiles into rings;
-//   warp 1     issues the MMAs. Per query tile X: S_X = Q_X K_t^T -> TMEM [256X, +128) fp32; P_X, written there by
-//              the softmax warps as 16-bit pairs over S_X, is the A operand of O_X += P_X V_t -> TMEM
-//              [256X + 128, +D). Order at key tile t: PV_A(t) S_A(t+1) PV_B(t) S_B(t+1), so the tensor core
-//              works on one query tile while the other's softmax runs;
-//   warps 4-11 softmax, one query row per thread (4-7 tile A, 8-11 tile B).
-// S_X(t+1) is issued after PV_X(t) and the MMAs of a CTA complete in order, so a softmax warp that sees S_X(t+1) may
-// overwrite P_X and rescale O_X. P is at most 2^8 (the running maximum is only replaced when it grows by more
-// than that) and is rounded to 16 bits for the product (half a step, relative); the row sum l adds the
-// unrounded fp32 values, the maximum, l and O stay in fp32.
+//   warp 0     takes items, hands them to the other warps through a two-slot ring, and loads K and V tiles (TMA) into
+//              rings;
+//   warp 1     issues the MMAs, by blocks of 64 keys with two score sets (set s = t % 2). Per query tile X: S_X = Q_X K_t^T
+//              -> TMEM [256X + 64s, +64) fp32; P_X, written there by the softmax warps as 16-bit pairs over S_X, is
+//              the A operand of O_X += P_X V_t -> TMEM [256X + 128, +D). Order: PV_X(t), S_X(t+2), so the scores of
+//              block t + 1 stand ready while t's softmax runs, and neither waits for the other;
+//   warp 3     loads the Q tiles, one lane each;
+//   warps 4-11 softmax, one query row per thread (4-7 tile A, 8-11 tile B), and the output through shared memory.
+// The two tiles meet only in the K and V rings (a slot is free when both have passed it) and the issuing thread
+// takes whichever is ready, so one may be in its next item while the other finishes: with short sequences an
+// item is few blocks, and what it costs to start and to end one (loads, output) hides behind the other tile's
+// work.
+// P is at most 2^8 (the running maximum is only replaced when it grows by more than that) and is rounded to 16
+// bits for the product (half a step, relative); the row sum l adds the unrounded fp32 values, the maximum, l and
+// O stay in fp32.
 constexpr uint64_t kBudgetNs = 2000000000ull, kDrainNs = 100000000ull;
-constexpr int BT = 128;  // rows of a query tile, keys of a key tile
-constexpr int kAtom = BT * 128;  // 128 rows x 128 bytes, one 128-byte-swizzle atom column of a tile
+constexpr int BT = 128;  // rows of a query tile (forward, dQ), keys of a tile (dK/dV)
+constexpr int BB = 64;   // keys (forward, dQ) or queries (dK/dV) of a block
+constexpr int kAtom = BT * 128;   // 128 rows x 128 bytes, one 128-byte-swizzle atom column of a tile
+constexpr int kAtom64 = BB * 128;  // and of a block
+
+// 32 columns of 32 rows on their way to memory: each lane writes its row into the warp's buffer (64-byte rows, 16-byte
+// pieces swizzled as the tensor map has it), then one lane sends it off. Rows behind the tensor's end are cut off.
+constexpr int kOutBytes = 32 * 64;
+__device__ __forceinline__ void out_piece(uint8_t* buf, int lane, int piece, uint4 v) {
+  *reinterpret_cast<uint4*>(buf + lane * 64 + ((piece ^ ((lane >> 1) & 3)) << 4)) = v;
+}
+__device__ __forceinline__ void out_send(const CUtensorMap* m, bool swap, const uint8_t* buf, int col, int head, int row) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_u32(buf)), "r"(col), "r"(swap ? row : head), "r"(swap ? head : row)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void out_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void out_wait_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 template <int D>
 struct FwdCfg {
-  static constexpr int kTile = BT * D * 2;
-  static constexpr int kK = D == 128 ? 3 : 4;  // ring depths: K runs one tile ahead of V
-  static constexpr int kV = D == 128 ? 2 : 4;
-  static constexpr int oQ = 0, oK = 2 * kTile, oV = oK + kK * kTile, oBar = oV + kV * kTile;
-  static constexpr int kSmem = oBar + 384 + 1024;
+  static constexpr int kTile = BT * D * 2, kBlock = BB * D * 2;
+  static constexpr int kK = 5, kV = 4;  // ring depths: K runs two blocks ahead of V
+  static constexpr int oQ = 0, oK = 2 * kTile, oV = oK + kK * kBlock;
+  static constexpr int oOut = oV + kV * kBlock;  // [8 warps] 32 rows x 32 columns of output on their way
+  static constexpr int oBar = oOut + 8 * kOutBytes;
+  static constexpr int kSmem = oBar + 448 + 1024;
   static_assert(kSmem <= 232448, "forward shared memory");
 };
 
 struct FwdMaps {
-  CUtensorMap q, k, v;
-  int swap;  // bit 0: q's map has its coordinates as (d, row, head), bit 1: k's, bit 2: v's
+  CUtensorMap q, k, v, o;
+  int swap;    // bit 0: q's map has its coordinates as (d, row, head), bit 1: k's, bit 2: v's
+  int swap_o;  // the same of o's map, whose boxes are 32 rows
 };
 
 __device__ __forceinline__ void load_tile(const CUtensorMap* m, bool swap, uint64_t* bar, uint8_t* dst, int head, int row,
@@ -244,9 +268,10 @@ __device__ __forceinline__ void load_tile(const CUtensorMap* m, bool swap, uint6
     tma_load_3d(m, bar, dst + c * atom_bytes, 64 * c, swap ? row : head, swap ? head : row);
 }
 
-// The blocks of these kernels are three warpgroups, launched with 168 registers a thread (64512 of an SM's 65536):
-// the first one, which loads and issues, gives most of its share up and the two that hold a score row per
-// thread take it: 128 x (104 + 200 + 200) = 64512.
+constexpr int kThreads = 384;
+// The backward's blocks are three warpgroups, launched with 168 registers a thread (64512 of an SM's 65536): the first
+// one, which loads and issues, gives a part of its share up and the two that hold score rows take it:
+// 128 x (104 + 200 + 200) = 64512.
 __device__ __forceinline__ void few_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); }
 __device__ __forceinline__ void many_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); }
 
@@ -262,11 +287,10 @@ __device__ __forceinline__ uint64_t mn_major(const void* tile, uint32_t atom) {
 
 struct FwdItem {
   int h[2], q0[2];  // head and first row of the query tiles A and B
-  int lo[2], hi[2];  // key tiles [lo, hi) of each (empty: no such query tile)
+  int lo[2], hi[2];  // key blocks [lo, hi) of each (empty: no such query tile)
   int kvh;
-  __device__ bool uses(int x, int t) const { return t >= lo[x] && t < hi[x]; }
   __device__ int first() const { return hi[1] > lo[1] ? min(lo[0], lo[1]) : lo[0]; }
-  __device__ int last() const { return max(hi[0], hi[1]); }  // one past the last key tile
+  __device__ int last() const { return max(hi[0], hi[1]); }  // one past the last key block
 };
 
 // where an item's query tiles are; the key ranges follow from the spans (item_keys) or the ring
@@ -286,71 +310,78 @@ __device__ __forceinline__ FwdItem item_rows(int block, int n_blocks, const Pack
   }
   I.kvh = I.h[0] / group;
   for (int x = 0; x < 2; ++x) {
-    I.hi[x] = I.q0[x] < p.N ? I.q0[x] / BT + 1 : 0;
+    I.hi[x] = I.q0[x] < p.N ? (min(I.q0[x] + BT, p.N) - 1) / BB + 1 : 0;
     I.lo[x] = 0;
   }
   return I;
 }
-// spans never decrease along the rows, so a tile's first row has its first key
-__device__ __forceinline__ void item_keys(FwdItem& I, const PackedParams& p) {
-  for (int x = 0; x < 2; ++x) I.lo[x] = I.hi[x] > 0 ? min(max(keys_of(p, I.q0[x]).x, 0) / BT, I.hi[x] - 1) : 0;
+// spans never decrease along the rows, so a tile's first row has its first key; returns the first row of the first
+// sequence: keys before it are foreign to every row of the item
+__device__ __forceinline__ int item_keys(FwdItem& I, const PackedParams& p) {
+  for (int x = 0; x < 2; ++x) I.lo[x] = I.hi[x] > 0 ? min(max(keys_of(p, I.q0[x]).x, 0) / BB, I.q0[x] / BB) : 0;
+  return __ldg(p.start + I.q0[0]);
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(384, 1) fwd_tc_kernel(const __grid_constant__ FwdMaps maps,
+__global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_constant__ FwdMaps maps,
                                                         const __grid_constant__ PackedParams p, int* status) {
   using C = FwdCfg<D>;
   constexpr int kAtoms = D / 64;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
-  uint64_t* q_full = bars + 0;
-  uint64_t* q_empty = bars + 1;
-  uint64_t* s_full = bars + 2;      // [2] per query tile
-  uint64_t* p_full = bars + 4;      // [2]
-  uint64_t* o_done = bars + 6;      // [2]
-  uint64_t* o_empty = bars + 8;     // [2]
-  uint64_t* item_full = bars + 10;  // [2] ring slots
-  uint64_t* item_empty = bars + 12;
-  uint64_t* drain = bars + 14;
-  uint64_t* clc_full = bars + 15;
-  uint64_t* k_full = bars + 16;
+  uint64_t* q_full = bars + 0;      // [2] per query tile
+  uint64_t* q_empty = bars + 2;     // [2]
+  uint64_t* s_full = bars + 4;      // [2][2] per query tile and score set
+  uint64_t* p_full = bars + 8;      // [2][2]
+  uint64_t* pv_done = bars + 12;    // [2] after each block's product with V
+  uint64_t* o_done = bars + 48;     // [2] after an item's last one
+  uint64_t* o_empty = bars + 14;    // [2]
+  uint64_t* item_full = bars + 16;  // [2] ring slots
+  uint64_t* item_empty = bars + 18;
+  uint64_t* drain = bars + 20;
+  uint64_t* clc_full = bars + 21;
+  uint64_t* k_full = bars + 22;
   uint64_t* k_empty = k_full + C::kK;
   uint64_t* v_full = k_empty + C::kK;
   uint64_t* v_empty = v_full + C::kV;
-  static_assert(16 + 2 * (C::kK + C::kV) <= 32, "barrier region");
-  volatile int* ring = reinterpret_cast<volatile int*>(bars + 32);  // [2][4]: block (-1: the end), lo of A, lo of B
-  uint8_t* clc_resp = reinterpret_cast<uint8_t*>(bars + 36);      // 16 bytes
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
+  static_assert(22 + 2 * (C::kK + C::kV) <= 40, "barrier region");
+  // [2][4]: block (-1: the end), first key block of A and of B, first row of A's first sequence
+  volatile int* ring = reinterpret_cast<volatile int*>(bars + 40);
+  uint8_t* clc_resp = reinterpret_cast<uint8_t*>(bars + 44);  // 16 bytes
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 46);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = warp_id();
   if (device_failed(status)) return;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 128);
+      mbar_init(&q_full[x], 1);
+      mbar_init(&q_empty[x], 1);
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(&s_full[2 * x + s], 1);
+        mbar_init(&p_full[2 * x + s], 128);
+      }
+      mbar_init(&pv_done[x], 1);
       mbar_init(&o_done[x], 1);
       mbar_init(&o_empty[x], 128);
       mbar_init(&item_full[x], 1);
-      mbar_init(&item_empty[x], 9);  // the MMA thread and one lane of each softmax warp
+      mbar_init(&item_empty[x], 12);  // the MMA thread for each tile, two Q loaders, one lane of each softmax warp
     }
     mbar_init(drain, 1);
     mbar_init(clc_full, 1);
     for (int i = 0; i < C::kK; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], 2);  // both query tiles have passed
     }
     for (int i = 0; i < C::kV; ++i) {
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], 2);
     }
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  if (warp == 3) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -368,92 +399,197 @@ __global__ void __launch_bounds__(384, 1) fwd_tc_kernel(const __grid_constant__ 
   };
 
   if (warp == 0) {
-    few_registers();
     if (elect_one()) {
-      tma_prefetch_desc(&maps.q);
       tma_prefetch_desc(&maps.k);
       tma_prefetch_desc(&maps.v);
-      int ik = 0, iv = 0;  // K and V tiles loaded so far (ring positions)
-      int nq = 0, nc = 0;  // Q loads and requests for work
-      int block = blockIdx.x;
+      int ik = 0, iv = 0, nc = 0;  // K and V tiles loaded so far (ring positions), requests for work
       bool ok = true;
-      for (int n = 0;; ++n) {
-        const int slot = n & 1;
-        if (n >= 2 && !wait(&item_empty[slot], (n - 2) >> 1)) {
-          ok = false;
-          break;
+      auto publish = [&](int n, int block, FwdItem& I) {
+        volatile int* slot = ring + (n & 1) * 4;
+        slot[0] = block;
+        if (block >= 0) {
+          I = item_rows(block, gridDim.x, p);
+          slot[3] = item_keys(I, p);
+          slot[1] = I.lo[0];
+          slot[2] = I.lo[1];
         }
-        if (block < 0) {
-          ring[slot * 4] = -1;
-          mbar_arrive(&item_full[slot]);
-          break;
-        }
-        FwdItem I = item_rows(block, gridDim.x, p);
-        item_keys(I, p);
-        ring[slot * 4] = block;
-        ring[slot * 4 + 1] = I.lo[0];
-        ring[slot * 4 + 2] = I.lo[1];
-        mbar_arrive(&item_full[slot]);
+        mbar_arrive(&item_full[n & 1]);
+      };
+      FwdItem I, next;
+      int block = blockIdx.x;
+      publish(0, block, I);
+      for (int n = 0; ok && block >= 0; ++n, I = next) {
         fence_async_smem();  // the last answer has been read before the next one is written over it
         clc_request(clc_resp, clc_full);
         ++nc;
-        if (n > 0 && !wait(q_empty, n - 1)) {  // the previous item's score MMAs have read the Q tiles
-          ok = false;
-          break;
-        }
-        const int nx = I.hi[1] > 0 ? 2 : 1;
-        mbar_arrive_expect_tx(q_full, nx * C::kTile);
-        ++nq;
-        for (int x = 0; x < nx; ++x)
-          load_tile(&maps.q, maps.swap & 1, q_full, smem + C::oQ + x * C::kTile, I.h[x], I.q0[x], kAtoms, kAtom);
+        // the next item is handed out as soon as it is known, between this item's loads: the other warps fetch it
+        // before they write this one's output
+        bool known = false, told = false;
+        auto look_ahead = [&](bool now) {
+          if (!known) {
+            if (now ? !wait(clc_full, n) : !mbar_test(clc_full, n & 1)) return !now;
+            block = clc_block(clc_resp);
+            known = true;
+          }
+          if (!told) {
+            uint64_t* free = &item_empty[(n + 1) & 1];
+            if (n > 0 && (now ? !wait(free, (n - 1) >> 1) : !mbar_test(free, ((n - 1) >> 1) & 1))) return !now;
+            publish(n + 1, block, next);
+            told = true;
+          }
+          return true;
+        };
         const int t0 = I.first(), t1 = I.last();
-        for (int t = t0; ok && t <= t1; ++t) {  // K(t0), then K(t+1) and V(t) in turn
+        for (int t = t0; ok && t < t1 + 2; ++t) {  // K(t0), K(t0+1), then K(t+2) and V(t) in turn
           if (t < t1) {
             const int st = ik % C::kK;
             if (!wait(&k_empty[st], (ik / C::kK) ^ 1)) {
               ok = false;
               break;
             }
-            mbar_arrive_expect_tx(&k_full[st], C::kTile);
-            load_tile(&maps.k, maps.swap & 2, &k_full[st], smem + C::oK + st * C::kTile, I.kvh, t * BT, kAtoms, kAtom);
+            mbar_arrive_expect_tx(&k_full[st], C::kBlock);
+            load_tile(&maps.k, maps.swap & 2, &k_full[st], smem + C::oK + st * C::kBlock, I.kvh, t * BB, kAtoms, kAtom64);
             ++ik;
           }
-          if (t > t0) {
+          if (t >= t0 + 2) {
             const int st = iv % C::kV;
             if (!wait(&v_empty[st], (iv / C::kV) ^ 1)) {
               ok = false;
               break;
             }
-            mbar_arrive_expect_tx(&v_full[st], C::kTile);
-            load_tile(&maps.v, maps.swap & 4, &v_full[st], smem + C::oV + st * C::kTile, I.kvh, (t - 1) * BT, kAtoms,
-                      kAtom);
+            mbar_arrive_expect_tx(&v_full[st], C::kBlock);
+            load_tile(&maps.v, maps.swap & 4, &v_full[st], smem + C::oV + st * C::kBlock, I.kvh, (t - 2) * BB, kAtoms,
+                      kAtom64);
             ++iv;
+            look_ahead(false);
           }
         }
-        if (!ok || !wait(clc_full, n)) {
-          ok = false;
-          break;
-        }
-        block = clc_block(clc_resp);
+        ok = ok && look_ahead(true);
       }
       if (!ok) {
         fail(kErrTimeoutProducer);
         // the copies in flight still write to this block's shared memory
         for (int g = max(0, ik - C::kK); g < ik; ++g) mbar_wait(&k_full[g % C::kK], (g / C::kK) & 1, kDrainNs, nullptr);
         for (int g = max(0, iv - C::kV); g < iv; ++g) mbar_wait(&v_full[g % C::kV], (g / C::kV) & 1, kDrainNs, nullptr);
-        if (nq > 0) mbar_wait(q_full, (nq - 1) & 1, kDrainNs, nullptr);
         if (nc > 0) mbar_wait(clc_full, (nc - 1) & 1, kDrainNs, nullptr);
       }
     }
   } else if (warp == 1) {
-    few_registers();
     if (elect_one()) {
-      constexpr uint32_t idesc_s = umma_idesc_16<T>(BT, BT, false, false);
+      constexpr uint32_t idesc_s = umma_idesc_16<T>(BT, BB, false, false);
       constexpr uint32_t idesc_o = umma_idesc_16<T>(BT, D, false, true);
-      int kbase = 0, vbase = 0;            // ring positions of the item's first K and V tiles
-      int pc[2] = {0, 0}, oc[2] = {0, 0};  // per query tile: P blocks consumed, items whose O is complete
+      // where a query tile is: at key block t (its product with V, then the scores of t + 2) of its n-th item [t0, t1),
+      // of which it uses [lo, hi)
+      struct Place {
+        int n, t, t0, t1, lo, hi;
+        int kpos, vpos;  // ring positions of the next K and V block
+        int nq;          // items begun
+        uint32_t np;     // bit s: parity of the uses of score set s
+        bool open, pv;   // in an item; the product with V_t (or its passing) is done
+        bool end;
+      };
+      Place pl[2] = {};
+      // the tile's next product, if what it needs is there; true if something was done
+      auto step = [&](auto xc) {
+        constexpr int x = decltype(xc)::value;
+        Place& w = pl[x];
+        const uint32_t tm = tmem + x * 256;
+        if (w.end) return false;
+        if (!w.open) {
+          const int slot = w.n & 1;
+          if (!mbar_test(&item_full[slot], (w.n >> 1) & 1)) return false;
+          if (ring[slot * 4] < 0) {
+            w.end = true;
+            return true;
+          }
+          const FwdItem I = item_of(slot);
+          mbar_arrive(&item_empty[slot]);
+          w.t0 = I.first(), w.t1 = I.last(), w.lo = I.lo[x], w.hi = I.hi[x];
+          w.t = w.t0 - 2;
+          w.open = true;
+          w.pv = false;
+        }
+        bool any = false;
+        if (!w.pv && w.t >= w.t0) {
+          const int t = w.t, st = w.vpos % C::kV, set = t & 1;
+          if (!mbar_test(&v_full[st], (w.vpos / C::kV) & 1)) return false;
+          if (t >= w.lo && t < w.hi) {  // O += P V_t; an item's first one overwrites O when the last item's has been read
+            if (!mbar_test(&p_full[2 * x + set], (w.np >> set) & 1)) return false;
+            if (t == w.lo && w.nq > 1 && !mbar_test(&o_empty[x], (w.nq - 2) & 1)) return false;
+            w.np ^= 1u << set;
+            tc_fence_after();
+            const uint64_t v_desc = mn_major(smem + C::oV + st * C::kBlock, kAtom64);
+#pragma unroll
+            for (int kk = 0; kk < BB / 16; ++kk)
+              umma_bf16_ts(tm + 128, tm + set * 64 + kk * 8, v_desc + kk * (2048 >> 4), idesc_o,
+                           (t > w.lo || kk > 0) ? 1u : 0u);
+            umma_commit(&v_empty[st]);
+            umma_commit(&pv_done[x]);
+            if (t == w.hi - 1) umma_commit(&o_done[x]);
+          } else {
+            mbar_arrive(&v_empty[st]);
+          }
+          ++w.vpos;
+          any = true;
+        }
+        w.pv = true;
+        if (w.t + 2 < w.t1) {
+          const int t = w.t + 2, st = w.kpos % C::kK, set = t & 1;
+          if (!mbar_test(&k_full[st], (w.kpos / C::kK) & 1)) return any;
+          if (t >= w.lo && t < w.hi) {  // S = Q K_t^T
+            if (t == w.lo) {
+              if (!mbar_test(&q_full[x], w.nq & 1)) return any;
+              ++w.nq;
+            }
+            tc_fence_after();
+            const uint64_t q_desc = k_major(smem + C::oQ + x * C::kTile), k_desc = k_major(smem + C::oK + st * C::kBlock);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t offq = ((kk >> 2) * kAtom + (kk & 3) * 32) >> 4, offk = ((kk >> 2) * kAtom64 + (kk & 3) * 32) >> 4;
+              umma_bf16_ss(tm + set * 64, q_desc + offq, k_desc + offk, idesc_s, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(&s_full[2 * x + set]);
+            umma_commit(&k_empty[st]);
+            if (t == w.hi - 1) umma_commit(&q_empty[x]);  // the item's last score product
+          } else {
+            mbar_arrive(&k_empty[st]);
+          }
+          ++w.kpos;
+        }
+        w.pv = false;
+        if (++w.t == w.t1) {
+          w.open = false;
+          ++w.n;
+        }
+        return true;
+      };
+      uint64_t since = globaltimer_ns();
       bool ok = true;
-      for (int n = 0; ok; ++n) {
+      for (uint32_t spin = 0; !(pl[0].end && pl[1].end);) {
+        const bool a = step(std::integral_constant<int, 0>{}), b = step(std::integral_constant<int, 1>{});
+        if (a || b) {
+          spin = 0;
+        } else if ((++spin & 255u) == 0) {
+          if (spin == 256) since = globaltimer_ns();
+          if (*abort_flag || (status && *reinterpret_cast<const volatile int*>(status)) ||
+              globaltimer_ns() - since > kBudgetNs) {
+            ok = false;
+            break;
+          }
+        }
+      }
+      if (!ok) fail(kErrTimeoutMma);
+      umma_commit(drain);
+      mbar_wait(drain, 0, kDrainNs, nullptr);
+    }
+  } else if (warp == 2) {
+  } else if (warp == 3) {
+    const int x = lane_id();
+    if (x < 2) {
+      tma_prefetch_desc(&maps.q);
+      int nq = 0;
+      bool ok = true;
+      for (int n = 0;; ++n) {
         const int slot = n & 1;
         if (!wait(&item_full[slot], n >> 1)) {
           ok = false;
@@ -462,143 +598,124 @@ __global__ void __launch_bounds__(384, 1) fwd_tc_kernel(const __grid_constant__ 
         if (ring[slot * 4] < 0) break;
         const FwdItem I = item_of(slot);
         mbar_arrive(&item_empty[slot]);
-        const int t0 = I.first(), t1 = I.last();
-        int scores = I.hi[0] - I.lo[0] + I.hi[1] - I.lo[1];  // score products of the item still to issue
-        ok = wait(q_full, n);
-        auto issue_s = [&](int x, int t) -> bool {  // S_X = Q_X K_t^T
-          const int g = kbase + t - t0, st = g % C::kK;
-          if (!wait(&k_full[st], g / C::kK)) return false;
-          tc_fence_after();
-          const uint64_t q_desc = k_major(smem + C::oQ + x * C::kTile), k_desc = k_major(smem + C::oK + st * C::kTile);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = ((kk >> 2) * kAtom + (kk & 3) * 32) >> 4;
-            umma_bf16_ss(tmem + x * 256, q_desc + off, k_desc + off, idesc_s, kk > 0 ? 1u : 0u);
-          }
-          umma_commit(&s_full[x]);
-          if (x == 1 || !I.uses(1, t)) umma_commit(&k_empty[st]);  // the tile's last reader
-          if (--scores == 0) umma_commit(q_empty);
-          return true;
-        };
-        auto issue_pv = [&](int x, int t) -> bool {  // O_X += P_X V_t
-          const int g = vbase + t - t0, st = g % C::kV;
-          // the first product of an item overwrites O: the softmax warps have read the previous item's
-          if (t == I.lo[x] && oc[x] > 0 && !wait(&o_empty[x], oc[x] - 1)) return false;
-          if (!wait(&p_full[x], pc[x]) || !wait(&v_full[st], g / C::kV)) return false;
-          ++pc[x];
-          tc_fence_after();
-          const uint64_t v_desc = mn_major(smem + C::oV + st * C::kTile, kAtom);
-#pragma unroll
-          for (int kk = 0; kk < BT / 16; ++kk)
-            umma_bf16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, v_desc + kk * (2048 >> 4), idesc_o,
-                         (t > I.lo[x] || kk > 0) ? 1u : 0u);
-          if (x == 1 || !I.uses(1, t)) umma_commit(&v_empty[st]);
-          if (t == I.hi[x] - 1) {
-            umma_commit(&o_done[x]);
-            ++oc[x];
-          }
-          return true;
-        };
-        for (int t = t0 - 1; ok && t < t1; ++t) {
-          for (int x = 0; x < 2 && ok; ++x) {
-            if (I.uses(x, t)) ok = issue_pv(x, t);
-            if (ok && I.uses(x, t + 1)) ok = issue_s(x, t + 1);
-          }
+        if ((x ? I.hi[1] : I.hi[0]) == 0) continue;
+        if (nq > 0 && !wait(&q_empty[x], nq - 1)) {  // the previous item's score products have read the tile
+          ok = false;
+          break;
         }
-        kbase += t1 - t0;
-        vbase += t1 - t0;
+        mbar_arrive_expect_tx(&q_full[x], C::kTile);
+        load_tile(&maps.q, maps.swap & 1, &q_full[x], smem + C::oQ + x * C::kTile, x ? I.h[1] : I.h[0],
+                  x ? I.q0[1] : I.q0[0], kAtoms, kAtom);
+        ++nq;
       }
-      if (!ok) fail(kErrTimeoutMma);
-      umma_commit(drain);
-      mbar_wait(drain, 0, kDrainNs, nullptr);
+      if (!ok) {
+        fail(kErrTimeoutProducer);
+        if (nq > 0) mbar_wait(&q_full[x], (nq - 1) & 1, kDrainNs, nullptr);
+      }
     }
-  } else if (warp < 4) {
-    few_registers();
+    __syncwarp();
   } else {
-    many_registers();
     const int x = (warp - 4) >> 2, wq = warp & 3, lane = lane_id();
     const int r = wq * 32 + lane;  // row of the tile = TMEM lane
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16) + x * 256;
-    int sc = 0, oc = 0;  // score blocks consumed and items finished by this query tile
-    int vbase = 0;       // ring position of the item's first V tile
-    for (int n = 0;; ++n) {
+    uint32_t sc = 0;  // bit s: parity of the uses of score set s
+    int pv = 0, oc = 0;  // this query tile's products with V, and its finished items, so far
+    int vbase = 0;    // ring position of the item's first V block
+    uint8_t* out_buf = smem + C::oOut + (warp - 4) * kOutBytes;
+    // an item as this thread sees it; `next` is fetched before an item's output is written, so that the spans arrive
+    // meanwhile
+    struct Work {
+      int block, t_lo, t_hi, h, i, t0, z, vfirst;
+      int2 key;
+    } now, next;
+    auto fetch = [&](int n, Work& w) -> bool {
       const int slot = n & 1;
       if (!mbar_wait_warp(&item_full[slot], (n >> 1) & 1, kBudgetNs, abort_flag, status)) {
         fail(kErrTimeoutEpilogue);
-        break;
+        return false;
       }
-      if (ring[slot * 4] < 0) break;
-      int t_lo, t_hi, h, i, t0, z, vfirst = vbase;
-      {
-        const FwdItem I = item_of(slot);
-        t0 = I.first();
-        vbase += I.last() - t0;
-        z = __ldg(p.start + I.q0[0]);  // keys before it are foreign to every row of the item
-        t_lo = x ? I.lo[1] : I.lo[0];
-        t_hi = x ? I.hi[1] : I.hi[0];
-        h = x ? I.h[1] : I.h[0];
-        i = (x ? I.q0[1] : I.q0[0]) + r;
-      }
+      w.block = ring[slot * 4];
+      if (w.block < 0) return true;
+      const FwdItem I = item_of(slot);
+      w.z = ring[slot * 4 + 3];
+      w.t0 = I.first();
+      w.vfirst = vbase;
+      vbase += I.last() - w.t0;
+      w.t_lo = x ? I.lo[1] : I.lo[0];
+      w.t_hi = x ? I.hi[1] : I.hi[0];
+      w.h = x ? I.h[1] : I.h[0];
+      w.i = (x ? I.q0[1] : I.q0[0]) + r;
+      w.key = w.i < p.N ? keys_of(p, w.i) : make_int2(0, 0);
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[slot]);
-      const int2 key = i < p.N ? keys_of(p, i) : make_int2(0, 0);
-      // rows of V that this thread clears before the item's first product
-      const bool clears = x == 0 && t_lo == t0 && t0 * BT + r < z;
+      return true;
+    };
+    bool more = fetch(0, now);
+    for (int n = 0; more && now.block >= 0; ++n, now = next) {
+      const int t_lo = now.t_lo, t_hi = now.t_hi, h = now.h, i = now.i, t0 = now.t0, z = now.z, vfirst = now.vfirst;
+      const int2 key = now.key;
+      // rows of V that this thread clears before its first product (both query tiles do, neither waits for the other)
+      const bool clears = t_lo == t0 && r < BB && t0 * BB + r < z;
       float m_ref = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int t = t_lo; t < t_hi; ++t, ++sc) {
-        if (!mbar_wait_warp(&s_full[x], sc & 1, kBudgetNs, abort_flag, status)) {
+      for (int t = t_lo; t < t_hi; ++t) {
+        const int set = t & 1;
+        const uint32_t set_base = lane_base + set * 64;
+        if (!mbar_wait_warp(&s_full[2 * x + set], (sc >> set) & 1, kBudgetNs, abort_flag, status)) {
           fail(kErrTimeoutEpilogue);
           ok = false;
           break;
         }
+        sc ^= 1u << set;
         tc_fence_after();
-        const int k0 = t * BT;
-        const bool all = __all_sync(0xffffffffu, key.x <= k0 && key.y >= k0 + BT);  // no key of the tile is hidden
-        // P = exp2(S scale - m) with the maximum so far: one pass, in which the tile's own maximum is found beside the
-        // exponentials. Only where that exceeds the old one by more than 2^8 (and in the first tile) are the
-        // scores read again and the exponentials taken anew. P replaces S in TMEM once it stands.
-        uint32_t pk[64];
+        const int kx = key.x - t * BB, ky = key.y - t * BB;  // the row sees the keys [kx, ky) of the block
+        // P = exp2(S scale - m) with the maximum so far: one pass, in which the block's own maximum is found beside
+        // the exponentials. Only where that exceeds the old one by more than 2^8 are the scores read again and
+        // the exponentials taken anew (an item's first block finds its maximum beforehand). P replaces S once
+        // it stands.
+        uint32_t pk[32];
         float mx, add;
         auto pass = [&](bool first) {
-          uint32_t sr[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(lane_base + c * 32, sr[c]);
+          uint32_t sr[2][32];
+          tmem_ld32(set_base, sr[0]);
+          tmem_ld32(set_base + 32, sr[1]);
           tmem_ld_wait();
-          if (!all) {
+          if (!__all_sync(0xffffffffu, kx <= 0 && ky >= BB)) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const uint32_t vis = range_mask32(key.x - k0 - 32 * c, key.y - k0 - 32 * c);
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t vis = range_mask32(kx - 32 * c, ky - 32 * c);
 #pragma unroll
               for (int e = 0; e < 32; ++e) sr[c][e] = ((vis >> e) & 1u) ? sr[c][e] : 0xff800000u;
             }
           }
           float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          if (first) {
 #pragma unroll
-            for (int e = 0; e < BT; ++e) part[e & 3] = fmaxf(part[e & 3], __uint_as_float(sr[e >> 5][e & 31]));
-            m_ref = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * p.scale_log2;
-          }
+          for (int e = 0; e < BB; e += 2)
+            part[(e >> 1) & 3] = fmaxf(fmaxf(part[(e >> 1) & 3], __uint_as_float(sr[e >> 5][e & 31])),
+                                       __uint_as_float(sr[e >> 5][(e + 1) & 31]));
+          mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * p.scale_log2;
+          if (first) m_ref = mx;
           const float mref = m_ref == -INFINITY ? 0.f : m_ref;
           const uint64_t sc2 = f32x2(p.scale_log2, p.scale_log2), nm2 = f32x2(-mref, -mref);
           uint64_t l2[2] = {0, 0};
 #pragma unroll
-          for (int e = 0; e < BT; e += 2) {
+          for (int e = 0; e < BB; e += 2) {
             const float s0 = __uint_as_float(sr[e >> 5][e & 31]), s1 = __uint_as_float(sr[e >> 5][(e + 1) & 31]);
-            part[(e >> 1) & 3] = fmaxf(fmaxf(part[(e >> 1) & 3], s0), s1);
             const float2 y = f32x2_split(fma_f32x2(f32x2(s0, s1), sc2, nm2));
             const float p0 = exp2f(y.x), p1 = exp2f(y.y);
             l2[(e >> 1) & 1] = add_f32x2(l2[(e >> 1) & 1], f32x2(p0, p1));
             pk[e / 2] = Half16<T>::pack(p0, p1);
           }
-          mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * p.scale_log2;
           const float2 ls = f32x2_split(add_f32x2(l2[0], l2[1]));
           add = ls.x + ls.y;
         };
-        pass(t == t_lo);
-        // The rescale is decided per row, but tcgen05.ld/st are warp-collective: the warp rescales together
-        // when any of its rows needs it, the others by 1.
-        if (t > t_lo) {
+        if (t == t_lo) {
+          pass(true);
+        } else {
+          pass(false);
+          // The rescale is decided per row, but tcgen05.ld/st are warp-collective: the warp rescales together
+          // when any of its rows needs it, the others by 1, and after the last block's product with V (the one
+          // before that has completed: it was issued before these scores).
           const bool mine = mx > m_ref + 8.f;
           if (__any_sync(0xffffffffu, mine)) {
             float alpha = 1.f;
@@ -607,6 +724,12 @@ __global__ void __launch_bounds__(384, 1) fwd_tc_kernel(const __grid_constant__ 
               l *= alpha;
               m_ref = mx;
             }
+            if (!mbar_wait_warp(&pv_done[x], (pv - 1) & 1, kBudgetNs, abort_flag, status)) {
+              fail(kErrTimeoutEpilogue);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t v[32];
@@ -620,77 +743,96 @@ __global__ void __launch_bounds__(384, 1) fwd_tc_kernel(const __grid_constant__ 
           }
         }
         l += add;
-        tmem_st32(lane_base, *reinterpret_cast<const uint32_t(*)[32]>(pk));
-        tmem_st32(lane_base + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
+        ++pv;
+        tmem_st32(set_base, pk);
         if (t == t_lo && clears) {
           if (!wait(&v_full[vfirst % C::kV], vfirst / C::kV)) *abort_flag = 1;
-          uint4* row = reinterpret_cast<uint4*>(smem + C::oV + vfirst % C::kV * C::kTile + r * 128);
+          uint4* row = reinterpret_cast<uint4*>(smem + C::oV + vfirst % C::kV * C::kBlock + r * 128);
 #pragma unroll 1
-          for (int c = 0; c < D / 64 * 8; ++c) row[(c >> 3) * (kAtom / 16) + (c & 7)] = make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < D / 64 * 8; ++c) row[(c >> 3) * (kAtom64 / 16) + (c & 7)] = make_uint4(0, 0, 0, 0);
           fence_async_smem();
         }
         __syncwarp();
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&p_full[x]);
+        mbar_arrive(&p_full[2 * x + set]);
       }
-      if (!ok) break;
+      more = ok && fetch(n + 1, next);
+      if (!more) break;
       if (t_hi <= t_lo) continue;
       if (!mbar_wait_warp(&o_done[x], oc & 1, kBudgetNs, abort_flag, status)) {
         fail(kErrTimeoutEpilogue);
         break;
       }
+      ++oc;
       tc_fence_after();
       const bool real = key.y > key.x;
       const float inv = 1.f / l;
       float odd = 0.f;  // becomes NaN when a value of the row is no number
+      // whole warps of rows go through shared memory (rows behind the end are cut off); a warp with padding rows among
+      // its own stores each row by itself
+      const bool send = __all_sync(0xffffffffu, real || i >= p.N) && i - lane < p.N;
       T* orow = reinterpret_cast<T*>(p.o.p) + (int64_t)i * p.o.row + h * p.o.head;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
+        const int col = c * 32;
         uint32_t v[32];
-        tmem_ld32(lane_base + 128 + c * 32, v);
+        tmem_ld32(lane_base + 128 + col, v);
+        if (send && lane == 0) out_wait_read();  // the buffer's last contents are on their way
+        __syncwarp();
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float y = __uint_as_float(v[e]) * inv;
-          odd = fmaf(y, 0.f, odd);
-          v[e] = __float_as_uint(y);
-        }
-        if (real) {
+        for (int e = 0; e < 32; e += 8) {
+          float y[8];
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 o;
-            o.x = Half16<T>::pack(__uint_as_float(v[e + 0]), __uint_as_float(v[e + 1]));
-            o.y = Half16<T>::pack(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
-            o.z = Half16<T>::pack(__uint_as_float(v[e + 4]), __uint_as_float(v[e + 5]));
-            o.w = Half16<T>::pack(__uint_as_float(v[e + 6]), __uint_as_float(v[e + 7]));
-            *reinterpret_cast<uint4*>(orow + c * 32 + e) = o;
+          for (int u = 0; u < 8; ++u) {
+            y[u] = __uint_as_float(v[e + u]) * inv;
+            odd = fmaf(y[u], 0.f, odd);
           }
+          const uint4 o = make_uint4(Half16<T>::pack(y[0], y[1]), Half16<T>::pack(y[2], y[3]),
+                                     Half16<T>::pack(y[4], y[5]), Half16<T>::pack(y[6], y[7]));
+          if (send) {
+            out_piece(out_buf, lane, e / 8, o);
+          } else if (real) {
+            *reinterpret_cast<uint4*>(orow + col + e) = o;
+          }
+        }
+        if (c == D / 32 - 1) {
+          // O is read: the next item's first product of this tile may overwrite it
+          tc_fence_before();
+          mbar_arrive(&o_empty[x]);
+        }
+        if (send) {
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) out_send(&maps.o, maps.swap_o, out_buf, col, h, i);
         }
         __syncwarp();
       }
       if (real) p.lse[(int64_t)h * p.N + i] = (m_ref + log2f(l)) * kLn2;
-      // O is read: the next item's first product of this tile may overwrite it
-      tc_fence_before();
-      mbar_arrive(&o_empty[x]);
-      ++oc;
       // rows that are no numbers although their scores are, and whose tiles hold foreign keys that were not cleared
       bool again = real && odd != 0.f && l == l;
       if (again) {
-        const int first = x == 0 || t_lo == t0 ? max(t_lo * BT, z) : t_lo * BT;
-        again = __ldg(p.start + i) > first || __ldg(p.end + i) < t_hi * BT;
+        const int first = t_lo == t0 ? max(t_lo * BB, z) : t_lo * BB;
+        again = __ldg(p.start + i) > first || __ldg(p.end + i) < t_hi * BB;
       }
       uint32_t redo = __ballot_sync(0xffffffffu, again);
+      if (redo) {
+        if (lane == 0) out_wait_done();  // these rows' first values are in memory before the second ones
+        __syncwarp();
+      }
       while (redo) {
         const int b = __ffs((int)redo) - 1;
         redo &= redo - 1;
         fwd_row<T, D>(p, i - lane + b, h, lane);
       }
     }
+    if (lane == 0) out_wait_done();
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 3) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -704,9 +846,6 @@ __global__ void __launch_bounds__(384, 1) fwd_tc_kernel(const __grid_constant__ 
 // loads, computes and stores, the other's block goes through the tensor core. P and dS are rounded to 16 bits
 // for their products (half a step, relative to each entry); everything else is fp32. They are written over the
 // scores that they came from.
-constexpr int BB = 64;  // keys (dQ) or queries (dK/dV) of a block
-constexpr int kAtom64 = BB * 128;
-
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                    smem_u32(dst)),
@@ -761,7 +900,7 @@ struct DqMaps {
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(384, 1) dq_tc_kernel(const __grid_constant__ DqMaps maps,
+__global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constant__ DqMaps maps,
                                                        const __grid_constant__ PackedParams p, int* status) {
   using C = DqCfg<D>;
   constexpr int kAtoms = D / 64;
@@ -1035,7 +1174,7 @@ struct DkvMaps {
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(384, 1) dkv_tc_kernel(const __grid_constant__ DkvMaps maps,
+__global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_constant__ DkvMaps maps,
                                                         const __grid_constant__ PackedParams p, int* status) {
   using C = DkvCfg<D>;
   constexpr int kAtoms = D / 64;
@@ -1348,10 +1487,10 @@ PackedParams common_params(const char* what, const torch::Tensor& q, const torch
   return p;
 }
 
-// TMA maps of [rows, heads, D] tensors with boxes of box_rows rows of one head; bit i of the result: the i-th map's
+// TMA maps of [rows, heads, D] tensors with boxes of box_rows rows and box_cols columns of one head; bit i of the result: the i-th map's
 // coordinates are (d, row, head)
 template <size_t n>
-int tile_maps(const std::pair<const torch::Tensor*, CUtensorMap*> (&sides)[n], int box_rows) {
+int tile_maps(const std::pair<const torch::Tensor*, CUtensorMap*> (&sides)[n], int box_rows, int box_cols = 64) {
   int swap = 0;
   for (size_t i = 0; i < n; ++i) {
     const torch::Tensor& t = *sides[i].first;
@@ -1359,7 +1498,7 @@ int tile_maps(const std::pair<const torch::Tensor*, CUtensorMap*> (&sides)[n], i
     bool s = false;
     *sides[i].second = tma_map_head_rows(
         t.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r.p, t.size(2),
-        t.size(1), t.size(0), r.head, r.row, box_rows, &s);
+        t.size(1), t.size(0), r.head, r.row, box_rows, &s, box_cols);
     swap |= (int)s << i;
   }
   return swap;
@@ -1408,8 +1547,10 @@ std::tuple<torch::Tensor, torch::Tensor> packed_attn_fwd(const torch::Tensor& q,
     constexpr int D = d();
     using C = FwdCfg<D>;
     FwdMaps maps;
-    const std::pair<const torch::Tensor*, CUtensorMap*> sides[] = {{&q, &maps.q}, {&k, &maps.k}, {&v, &maps.v}};
-    maps.swap = tile_maps(sides, BT);
+    const std::pair<const torch::Tensor*, CUtensorMap*> q_side[] = {{&q, &maps.q}}, kv_side[] = {{&k, &maps.k}, {&v, &maps.v}},
+                                                        to[] = {{&out, &maps.o}};
+    maps.swap = tile_maps(q_side, BT) | tile_maps(kv_side, BB) << 1;
+    maps.swap_o = tile_maps(to, 32, 32);
     once_per_device(q.device().index(), [] {
       C10_CUDA_CHECK(cudaFuncSetAttribute(fwd_tc_kernel<decltype(t), D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           C::kSmem));
@@ -1417,7 +1558,7 @@ std::tuple<torch::Tensor, torch::Tensor> packed_attn_fwd(const torch::Tensor& q,
     const int64_t tiles = (p.N + BT - 1) / BT;
     const int64_t items = p.H / p.KV % 2 == 0 ? tiles * (p.H / 2) : (tiles + 1) / 2 * p.H;
     TORCH_CHECK_VALUE(items < (int64_t(1) << 31), what, ": too many rows or heads");
-    fwd_tc_kernel<decltype(t), D><<<(unsigned)items, 384, C::kSmem, st>>>(maps, p, status_ptr(q.device().index()));
+    fwd_tc_kernel<decltype(t), D><<<(unsigned)items, kThreads, C::kSmem, st>>>(maps, p, status_ptr(q.device().index()));
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {out, lse};
@@ -1477,9 +1618,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
     const int64_t tiles = p.Np / BT;
     TORCH_CHECK_VALUE(tiles * H < (int64_t(1) << 31), what, ": too many rows or heads");
     int* status = status_ptr(q.device().index());
-    dq_tc_kernel<T, D><<<(unsigned)(tiles * H), 384, DqCfg<D>::kSmem, st>>>(a, p, status);
+    dq_tc_kernel<T, D><<<(unsigned)(tiles * H), kThreads, DqCfg<D>::kSmem, st>>>(a, p, status);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
-    dkv_tc_kernel<T, D><<<(unsigned)(tiles * KV), 384, DkvCfg<D>::kSmem, st>>>(b, p, status);
+    dkv_tc_kernel<T, D><<<(unsigned)(tiles * KV), kThreads, DkvCfg<D>::kSmem, st>>>(b, p, status);
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {dq, dk, dv};

@@ -44,20 +44,21 @@ inline CUtensorMap tma_map_3d(CUtensorMapDataType dtype, int elem_bytes, const v
   return m;
 }
 
-// Tiles of rows x 64 elements of one head of a [rows, heads, D] tensor of 16-bit values (strides in elements,
+// Tiles of rows x box_cols elements (64: 128-byte swizzle, 32: 64-byte) of one head of a [rows, heads, D] tensor of 16-bit values (strides in elements,
 // multiples of 8): a 3-D map whose dimensions stand in the order of their strides. `swapped`: the coordinates are
 // (d, row, head) instead of (d, head, row).
 inline CUtensorMap tma_map_head_rows(CUtensorMapDataType dtype, const void* base, int64_t D, int64_t heads, int64_t rows,
-                                     int64_t head_stride, int64_t row_stride, int box_rows, bool* swapped) {
+                                     int64_t head_stride, int64_t row_stride, int box_rows, bool* swapped, int box_cols = 64) {
   *swapped = head_stride > row_stride;
   CUtensorMap m;
   cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)(*swapped ? rows : heads), (cuuint64_t)(*swapped ? heads : rows)};
   cuuint64_t strides[2] = {(cuuint64_t)(2 * (*swapped ? row_stride : head_stride)),
                            (cuuint64_t)(2 * (*swapped ? head_stride : row_stride))};
-  cuuint32_t box[3] = {64, (cuuint32_t)(*swapped ? box_rows : 1), (cuuint32_t)(*swapped ? 1 : box_rows)};
+  cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)(*swapped ? box_rows : 1), (cuuint32_t)(*swapped ? 1 : box_rows)};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = tma_encode_fn()(&m, dtype, 3, const_cast<void*>(base), dims, strides, box, estr,
-                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed: ", std::to_string((int)r));
   return m;
