@@ -853,29 +853,40 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// 32 fp32 columns of a TMEM row, times f, to 32 16-bit values in memory; true if one of them is no number
+// 32 fp32 columns of this warp's 32 TMEM rows, times f, as 16-bit values to columns [col, +32) of head `head` of rows
+// i (one per lane); true in a lane whose row has a value that is no number. Whole warps of rows go through the
+// warp's buffer in shared memory, a warp with rows that are not written among its own stores each by itself.
 template <typename T>
-__device__ __forceinline__ bool store_cols(uint32_t taddr, float f, T* dst, bool write) {
+__device__ __forceinline__ bool store_cols(uint32_t taddr, float f, const Rows& to, const CUtensorMap* map, bool swap,
+                                           uint8_t* buf, int col, int head, int i, int lane, bool write, int N) {
   uint32_t v[32];
   tmem_ld32(taddr, v);
+  const bool send = __all_sync(0xffffffffu, write || i >= N) && i - lane < N;
+  T* dst = reinterpret_cast<T*>(to.p) + (int64_t)i * to.row + head * to.head + col;
+  if (send && lane == 0) out_wait_read();
+  __syncwarp();
   tmem_ld_wait();
   float odd = 0.f;
 #pragma unroll
-  for (int e = 0; e < 32; ++e) {
-    const float y = __uint_as_float(v[e]) * f;
-    odd = fmaf(y, 0.f, odd);
-    v[e] = __float_as_uint(y);
-  }
-  if (write) {
+  for (int e = 0; e < 32; e += 8) {
+    float y[8];
 #pragma unroll
-    for (int e = 0; e < 32; e += 8) {
-      uint4 o;
-      o.x = Half16<T>::pack(__uint_as_float(v[e + 0]), __uint_as_float(v[e + 1]));
-      o.y = Half16<T>::pack(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
-      o.z = Half16<T>::pack(__uint_as_float(v[e + 4]), __uint_as_float(v[e + 5]));
-      o.w = Half16<T>::pack(__uint_as_float(v[e + 6]), __uint_as_float(v[e + 7]));
+    for (int u = 0; u < 8; ++u) {
+      y[u] = __uint_as_float(v[e + u]) * f;
+      odd = fmaf(y[u], 0.f, odd);
+    }
+    const uint4 o = make_uint4(Half16<T>::pack(y[0], y[1]), Half16<T>::pack(y[2], y[3]), Half16<T>::pack(y[4], y[5]),
+                               Half16<T>::pack(y[6], y[7]));
+    if (send) {
+      out_piece(buf, lane, e / 8, o);
+    } else if (write) {
       *reinterpret_cast<uint4*>(dst + e) = o;
     }
+  }
+  if (send) {
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) out_send(map, swap, buf, col, head, i);
   }
   __syncwarp();
   return odd != 0.f;
@@ -888,15 +899,18 @@ template <int D>
 struct DqCfg {
   static constexpr int kTile = BB * D * 2;
   static constexpr int kStages = 6;
-  static constexpr int oK = 0, oV = kStages * kTile, oSum = oV + kStages * kTile;  // oSum: [2][128] half-row sums
+  static constexpr int oK = 0, oV = kStages * kTile;
+  // the tile's Q and dO rows wait in the ring's stages 3 and 4 until they are in TMEM, its O rows by themselves
+  static constexpr int oQ = oK + 3 * kTile, oD = oV + 3 * kTile, oO = oV + kStages * kTile;
+  static constexpr int oSum = oO + 2 * kTile;  // [2][128] half-row sums
   static constexpr int oBar = oSum + 1024;
   static constexpr int kSmem = oBar + 256 + 1024;
   static_assert(kSmem <= 232448, "dQ shared memory");
 };
 
 struct DqMaps {
-  CUtensorMap k, v;
-  int swap;
+  CUtensorMap k, v, q, d, o, dq;
+  int swap_kv, swap_in, swap_dq;  // bits of swap_in: q, dO, O
 };
 
 template <typename T, int D>
@@ -913,7 +927,9 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
   uint64_t* p_full = bars + 4;  // [2]
   uint64_t* kv_full = bars + 6;
   uint64_t* kv_empty = kv_full + C::kStages;
-  static_assert(6 + 2 * C::kStages <= 28, "barrier region");
+  uint64_t* in_full = kv_empty + C::kStages;  // Q, dO and O have arrived
+  uint64_t* in_read = in_full + 1;            // Q and dO are in TMEM
+  static_assert(8 + 2 * C::kStages <= 28, "barrier region");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -927,6 +943,8 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
   const int nb = kb_hi - kb_lo + 1;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 256);  // every softmax thread has stored its Q or dO row in TMEM
+    mbar_init(in_full, 1);
+    mbar_init(in_read, 256);
     mbar_init(done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -953,21 +971,26 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
   if (warp == 0) {
     few_registers();
     if (elect_one()) {
+      mbar_arrive_expect_tx(in_full, 3 * BT * D * 2);
+      load_tile(&maps.q, maps.swap_in & 1, in_full, smem + C::oQ, h, q0, kAtoms, kAtom);
+      load_tile(&maps.d, maps.swap_in & 2, in_full, smem + C::oD, h, q0, kAtoms, kAtom);
+      load_tile(&maps.o, maps.swap_in & 4, in_full, smem + C::oO, h, q0, kAtoms, kAtom);
       int j = 0;
       bool ok = true;
       for (; j < nb; ++j) {
         const int st = j % C::kStages;
-        if (!wait(&kv_empty[st], (j / C::kStages) ^ 1)) {
+        if (!wait(&kv_empty[st], (j / C::kStages) ^ 1) || (j == 3 && !wait(in_read, 0))) {
           ok = false;
           break;
         }
         const int k0 = (kb_lo + j) * BB;
         mbar_arrive_expect_tx(&kv_full[st], 2 * C::kTile);
-        load_tile(&maps.k, maps.swap & 1, &kv_full[st], smem + C::oK + st * C::kTile, kvh, k0, kAtoms, kAtom64);
-        load_tile(&maps.v, maps.swap & 2, &kv_full[st], smem + C::oV + st * C::kTile, kvh, k0, kAtoms, kAtom64);
+        load_tile(&maps.k, maps.swap_kv & 1, &kv_full[st], smem + C::oK + st * C::kTile, kvh, k0, kAtoms, kAtom64);
+        load_tile(&maps.v, maps.swap_kv & 2, &kv_full[st], smem + C::oV + st * C::kTile, kvh, k0, kAtoms, kAtom64);
       }
       if (!ok) {
         fail(kErrTimeoutProducer);
+        mbar_wait(in_full, 0, kDrainNs, nullptr);
         for (int g = max(0, j - C::kStages); g < j; ++g)
           mbar_wait(&kv_full[g % C::kStages], (g / C::kStages) & 1, kDrainNs, nullptr);
       }
@@ -1018,60 +1041,58 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
   } else {
     many_registers();
     const int wq = warp & 3, lane = lane_id(), half = (warp - 4) >> 2;
-    const int r = wq * 32 + lane, i = q0 + r, ic = min(i, p.N - 1);
+    const int r = wq * 32 + lane, i = q0 + r;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16);
     const int2 key = i < p.N ? keys_of(p, i) : make_int2(0, 0);
     const bool real = key.y > key.x;
-    {
-      // this row's Q (first warp of the row) or dO (second warp) into TMEM: the A operands of S and dP
-      const Rows& src = half == 0 ? p.q : p.dout;
-      const uint4* g = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(src.p) + ic * src.row + h * src.head);
+    const float lse = real ? p.lse[(int64_t)h * p.N + i] * kLog2e : INFINITY;
+    bool ok = mbar_wait_warp(in_full, 0, kBudgetNs, abort_flag, status);
+    if (!ok) fail(kErrTimeoutEpilogue);
+    // 16 bytes, the piece-th of this row of a tile
+    auto piece_of = [&](int tile_at, int piece) {
+      return *reinterpret_cast<const uint4*>(smem + tile_at + (piece >> 3) * kAtom + r * 128 + (((piece & 7) ^ (r & 7)) << 4));
+    };
+    // this row's Q (first warp of the row) or dO (second warp) into TMEM: the A operands of S and dP
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t w[32];
+    for (int c = 0; c < D / 64; ++c) {
+      uint32_t w[32];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint4 a = __ldg(g + c * 8 + e);
-          w[4 * e] = a.x;
-          w[4 * e + 1] = a.y;
-          w[4 * e + 2] = a.z;
-          w[4 * e + 3] = a.w;
-        }
-        tmem_st32(lane_base + 384 + 64 * half + 32 * c, w);
+      for (int e = 0; e < 8; ++e) {
+        const uint4 a = piece_of(half == 0 ? C::oQ : C::oD, c * 8 + e);
+        w[4 * e] = a.x;
+        w[4 * e + 1] = a.y;
+        w[4 * e + 2] = a.z;
+        w[4 * e + 3] = a.w;
       }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(q_full);
+      tmem_st32(lane_base + 384 + 64 * half + 32 * c, w);
     }
+    tmem_st_wait();
+    tc_fence_before();
+    mbar_arrive(q_full);
     // delta: the two warps of a row each reduce half of its values and meet in shared memory
     float2 stat;
     {
       float* sums = reinterpret_cast<float*>(smem + C::oSum);
-      const uint4* og = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.o.p) + ic * p.o.row + h * p.o.head +
-                                                       half * (D / 2));
-      const uint4* dg = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.dout.p) + ic * p.dout.row +
-                                                       h * p.dout.head + half * (D / 2));
       float acc = 0.f;
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) {
-        const uint4 a = __ldg(og + e), b = __ldg(dg + e);
-        const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+        const uint4 a = piece_of(C::oO, half * (D / 16) + e), b = piece_of(C::oD, half * (D / 16) + e);
+        const uint32_t u[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float2 u = Half16<T>::unpack(x[k]), w = Half16<T>::unpack(y[k]);
-          acc = fmaf(u.x, w.x, fmaf(u.y, w.y, acc));
+          const float2 f = Half16<T>::unpack(u[k]), w = Half16<T>::unpack(y[k]);
+          acc = fmaf(f.x, w.x, fmaf(f.y, w.y, acc));
         }
       }
+      mbar_arrive(in_read);
       sums[half * 128 + r] = acc;
       asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps
-      stat = real ? make_float2(p.lse[(int64_t)h * p.N + i] * kLog2e, sums[r] + sums[128 + r])
-                  : make_float2(INFINITY, 0.f);
+      stat = make_float2(lse, real ? sums[r] + sums[128 + r] : 0.f);
       if (half == 0) p.stat[(int64_t)h * p.Np + i] = make_float2(-stat.x, -stat.y);
     }
     const int z = __ldg(p.start + q0);  // keys before it are foreign to every row of the tile: all in block kb_lo
-    bool ok = true;
     const uint32_t set_base = lane_base + half * 128;
-    for (int j = half; j < nb; j += 2) {
+    for (int j = half; ok && j < nb; j += 2) {
       if (!mbar_wait_warp(&s_full[half], (j >> 1) & 1, kBudgetNs, abort_flag, status)) {
         fail(kErrTimeoutEpilogue);
         ok = false;
@@ -1128,15 +1149,17 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     }
     if (ok && mbar_wait_warp(done, 0, kBudgetNs, abort_flag, status)) {
       tc_fence_after();
-      T* row = reinterpret_cast<T*>(p.dq.p) + (int64_t)i * p.dq.row + h * p.dq.head;
       bool odd = false;
 #pragma unroll 1
-      for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c)
-        odd |= store_cols<T>(lane_base + 256 + c * 32, p.scale, row + c * 32, real);
+      for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c)  // through the ring's memory, which is free by now
+        odd |= store_cols<T>(lane_base + 256 + c * 32, p.scale, p.dq, &maps.dq, maps.swap_dq,
+                             smem + C::oK + (warp - 4) * kOutBytes, c * 32, h, i, lane, real, p.N);
       // as in the forward: no number, though the scores are, and foreign keys among the tile's that were not cleared
       bool again = real && odd && stat.x == stat.x;
       if (again) again = __ldg(p.start + i) > max(kb_lo * BB, z) || __ldg(p.end + i) < (kb_hi + 1) * BB;
       uint32_t redo = __ballot_sync(0xffffffffu, again);
+      if (lane == 0) out_wait_done();  // also before any row's second values
+      __syncwarp();
       while (redo) {
         const int b = __ffs((int)redo) - 1;
         redo &= redo - 1;
@@ -1169,8 +1192,8 @@ struct DkvCfg {
 };
 
 struct DkvMaps {
-  CUtensorMap k, v, q, d;
-  int swap_kv, swap_qd;
+  CUtensorMap k, v, q, d, dv, dk;
+  int swap_kv, swap_qd, swap_o;  // bits of swap_o: dv, dk
 };
 
 template <typename T, int D>
@@ -1381,17 +1404,20 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     }
     if (ok && mbar_wait_warp(done, 0, kBudgetNs, abort_flag, status)) {
       tc_fence_after();
-      // half 0 writes dV, half 1 writes dK
+      // half 0 writes dV, half 1 dK, through the ring's memory, which is free by now
       const Rows& to = half ? p.dk : p.dv;
-      T* row = reinterpret_cast<T*>(to.p) + (int64_t)j * to.row + kvh * to.head;
       bool odd = false;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c)
-        odd |= store_cols<T>(lane_base + (half ? 384 : 256) + c * 32, half ? p.scale : 1.f, row + c * 32, real);
+        odd |= store_cols<T>(lane_base + (half ? 384 : 256) + c * 32, half ? p.scale : 1.f, to, half ? &maps.dk : &maps.dv,
+                             (maps.swap_o >> half) & 1, smem + C::oQ + (warp - 4) * kOutBytes, c * 32, kvh, j, lane, real,
+                             p.N);
       // no number, and foreign queries among the tile's that were not cleared
       bool again = real && odd;
       if (again) again = __ldg(p.start + j) > k0 || __ldg(p.end + j) < min(z, (qb_hi + 1) * BB);
       uint32_t redo = __ballot_sync(0xffffffffu, again);
+      if (lane == 0) out_wait_done();  // also before any row's second values
+      __syncwarp();
       while (redo) {
         const int b = __ffs((int)redo) - 1;
         redo &= redo - 1;
@@ -1606,11 +1632,16 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
     constexpr int D = d();
     DqMaps a;
     const std::pair<const torch::Tensor*, CUtensorMap*> kv64[] = {{&k, &a.k}, {&v, &a.v}};
-    a.swap = tile_maps(kv64, BB);
+    a.swap_kv = tile_maps(kv64, BB);
+    const std::pair<const torch::Tensor*, CUtensorMap*> in[] = {{&q, &a.q}, {&dout, &a.d}, {&out, &a.o}}, to_q[] = {{&dq, &a.dq}};
+    a.swap_in = tile_maps(in, BT);
+    a.swap_dq = tile_maps(to_q, 32, 32);
     DkvMaps b;
     const std::pair<const torch::Tensor*, CUtensorMap*> kv[] = {{&k, &b.k}, {&v, &b.v}}, qd[] = {{&q, &b.q}, {&dout, &b.d}};
     b.swap_kv = tile_maps(kv, BT);
     b.swap_qd = tile_maps(qd, BB);
+    const std::pair<const torch::Tensor*, CUtensorMap*> to_kv[] = {{&dv, &b.dv}, {&dk, &b.dk}};
+    b.swap_o = tile_maps(to_kv, 32, 32);
     once_per_device(q.device().index(), [] {
       C10_CUDA_CHECK(cudaFuncSetAttribute(dq_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DqCfg<D>::kSmem));
       C10_CUDA_CHECK(cudaFuncSetAttribute(dkv_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DkvCfg<D>::kSmem));
