@@ -201,8 +201,9 @@ class TrainConfig:
     token_bytes_max: int = 16
     bos_every: int = 64
     document_buffer_size: int = 1000
+    document_mask: bool = False  # attention stays inside documents: a BOS token starts a new one within a row
     documents_bos_prefixed: bool = False  # data=documents: the documents already start with BOS
-    bos_token_id: int = -1  # data=documents: -1 = vocab_size - 1
+    bos_token_id: int = -1  # data=documents and document_mask: -1 = vocab_size - 1
     # compute
     impl: str = "cuda"  # "cuda" (sm_100a kernels) or "torch" (eager oracle path)
     # impl=torch on a GPU: run the eager model under torch.compile with flex attention (a fused

@@ -31,8 +31,9 @@ from __future__ import annotations
 import torch
 
 from ..config import effective_window, has_value_embedding
-from ..ops import gemm
+from ..ops import gemm, packed
 from ..ops._ext import check_status, ext
+from ..ops.distill import Teacher, distill_topk
 from ..utils.timing import traced
 
 
@@ -75,6 +76,8 @@ class FusedGPTEngine:
         self.bucket_hook = None
         # tcgen05 attention needs 128-wide heads and whole 128-row tiles; otherwise the register-tiled kernels
         self.tc_attention = seq % 128 == 0 and self.hd == 128
+        # attention inside the documents of a row (a document starts at each token of this id): packed attention
+        self.document_bos = model.document_bos
         # the QKV GEMM applies RoPE/QK-norm/VE in its epilogue when each 256-column tile holds two heads
         self.fused_rope = self.hd == 128 and self.H % 2 == 0 and self.KV % 2 == 0
         self._hook_on = False
@@ -133,7 +136,8 @@ class FusedGPTEngine:
             "rk": [torch.empty(M, KV, **f32) for _ in range(L)],
             "gate": {i: torch.empty(M, KV, **f32) for i in self.ve_layers},
             "o": [torch.empty(M, D, **bf) for _ in range(L)],
-            "lse": [torch.empty(B, H, T, **f32) for _ in range(L)],
+            "lse": [torch.empty(H, M, **f32) if self.document_bos is not None else torch.empty(B, H, T, **f32)
+                    for _ in range(L)],
             "h": [torch.empty(M, self.F, **bf) for _ in range(L)],
             "rstdf": torch.empty(M, **f32), "xf": torch.empty(M, D, **bf),
             # fused head: G (dlogits up to a per-row scale and the target column), CE statistics
@@ -149,14 +153,31 @@ class FusedGPTEngine:
             "delta": torch.empty(B, H, T, **f32), "dz": torch.empty(M, KV, **f32),
             "dgate_in": torch.empty(M, 32, **f32), "dx0": torch.empty(M, D, **f32),
         }
+        if self.document_bos is not None:
+            i32 = dict(dtype=torch.int32, device=self.dev)
+            b["start"], b["end"] = torch.empty(M, **i32), torch.empty(M, **i32)
+            b["attn_scratch"] = torch.empty(packed.bwd_scratch(M, H), **f32)
         self.bufs[B] = b
         return b
+
+    def _heads(self, t: torch.Tensor, first: int, count: int) -> torch.Tensor:
+        """Heads [first, first + count) of a [M, heads * hd] buffer as [M, count, hd]."""
+        return t.unflatten(1, (-1, self.hd))[:, first:first + count]
+
+    def _qkv_heads(self, t: torch.Tensor):
+        H, KV = self.H, self.KV
+        return self._heads(t, 0, H), self._heads(t, H, KV), self._heads(t, H + KV, KV)
+
+    def _packed_window(self, i: int) -> int:
+        return self.windows[i] if self.windows[i] < self.T else 0
 
     # ------------------------------------------------------------------ forward
     def _forward(self, idx: torch.Tensor, b: dict, B: int):
         E, P = self.E, self.P
         T, D, H, KV, hd = self.T, self.D, self.H, self.KV, self.hd
         Dq, Dkv = self.Dq, self.Dkv
+        if self.document_bos is not None:  # the documents' spans, for every layer of both passes
+            packed.bounds_from_ids(idx.reshape(B, T), self.document_bos, b["start"], b["end"])
         idx = idx.reshape(-1)
         ready = self.param_ready or (lambda g: None)
         ready(0)
@@ -175,7 +196,10 @@ class FusedGPTEngine:
                 gemm.matmul(xn, self.wqkv[i], out=qkv)
                 E.rope_fwd(qkv, T, H, KV, hd, self.cos, self.sin, b["rq"][i], b["rk"][i], *ve_args)
             o = b["o"][i]
-            if self.tc_attention:
+            if self.document_bos is not None:
+                packed.attention_fwd(*self._qkv_heads(qkv), b["start"], b["end"], window=self._packed_window(i),
+                                     out=self._heads(o, 0, H), lse=b["lse"][i])
+            elif self.tc_attention:
                 E.attn_fwd_tc(qkv, o, b["lse"][i], B, T, H, KV, hd, self.windows[i])
             else:
                 E.attn_fwd(qkv[:, :Dq], qkv[:, Dq:Dq + Dkv], qkv[:, Dq + Dkv:], o, b["lse"][i], B, T, H, KV, hd,
@@ -203,8 +227,17 @@ class FusedGPTEngine:
         else:
             E.ce_finalize(b["ce_part"], b["zt"], tg, self.V, 15.0, scale, nats=b["nats"])
 
+    def _teacher_head(self, tg: torch.Tensor, b: dict, scale: float, teacher: Teacher):
+        """lm_head + softcap 15, then the loss against the teacher's top logits; G becomes its gradient with respect
+        to the scores before the softcap (the logits do reach memory here: the teacher's columns are read from them)."""
+        M = tg.numel()
+        gemm.matmul(b["xf"], self.shadows["lmHead"].t(), out=b["G"], epi=gemm.SOFTCAP, alpha=1.0 / 15.0, beta=15.0)
+        loss, _, _ = distill_topk(b["G"], teacher.ids.reshape(M, -1), teacher.logits.reshape(M, -1), tg, cap=15.0,
+                                  temperature=teacher.temperature, alpha=teacher.alpha, scale=scale, grad=b["G"])
+        b["loss"].copy_(loss)
+
     # ------------------------------------------------------------------ backward
-    def _backward(self, idx: torch.Tensor, tg: torch.Tensor, b: dict, B: int):
+    def _backward(self, idx: torch.Tensor, tg: torch.Tensor, b: dict, B: int, scaled: bool = True):
         E, P, G = self.E, self.P, self.grads
         T, D, H, KV, hd = self.T, self.D, self.H, self.KV, self.hd
         Dq, Dkv = self.Dq, self.Dkv
@@ -212,10 +245,11 @@ class FusedGPTEngine:
         A = gemm.ATOMIC
         # head: dlogits = rowscale * G (ce_finalize wrote the target column into G), so
         # dlmHead += G^T (rowscale xf) and dxf = rowscale (G lmHead), the scale folded into rms_bwd
-        gemm.matmul(b["G"].t(), b["xs_head"], out=G["lmHead"], epi=A, k_splits=0)
+        # (not ``scaled``: G is dlogits itself)
+        gemm.matmul(b["G"].t(), b["xs_head"] if scaled else b["xf"], out=G["lmHead"], epi=A, k_splits=0)
         gemm.matmul(b["G"], self.shadows["lmHead"], out=b["dmid"], epi=gemm.F32)
         self._ready(0)
-        E.rms_bwd(b["xs"][-1], b["rstdf"], b["dmid"], None, b["dx"], b["dx_b"], b["rowscale"])
+        E.rms_bwd(b["xs"][-1], b["rstdf"], b["dmid"], None, b["dx"], b["dx_b"], b["rowscale"] if scaled else None)
         b["dx0"].zero_()
         for i in reversed(range(self.L)):
             # MLP
@@ -230,7 +264,12 @@ class FusedGPTEngine:
             gemm.matmul(b["dmid_b"], self.shadows[f"layer{i}_proj"].t(), out=b["do"])
             qkv, dqkv = b["qkv"][i], b["dqkv"]
             ve = i in b["gate"]
-            if self.tc_attention:
+            if self.document_bos is not None:
+                dq, dk, dv = self._qkv_heads(dqkv)
+                packed.attention_bwd(*self._qkv_heads(qkv), self._heads(b["o"][i], 0, H), b["lse"][i],
+                                     self._heads(b["do"], 0, H), b["start"], b["end"], window=self._packed_window(i), dq=dq,
+                                     dk=dk, dv=dv, scratch=b["attn_scratch"])
+            elif self.tc_attention:
                 E.attn_bwd_tc(qkv, b["o"][i], b["do"], b["lse"][i], dqkv, b["delta"], B, T, H, KV, hd, self.windows[i])
             else:
                 E.attn_bwd(qkv[:, :Dq], qkv[:, Dq:Dq + Dkv], qkv[:, Dq + Dkv:], b["o"][i], b["do"], b["lse"][i],
@@ -262,8 +301,11 @@ class FusedGPTEngine:
 
     # ------------------------------------------------------------------ API
     def forward_backward(self, idx: torch.Tensor, targets: torch.Tensor, loss_scale: float = 1.0,
-                         accumulate: bool = False, last_micro: bool = True, grad_scale: float = 1.0) -> torch.Tensor:
-        """Accumulates gradients of ``loss_scale * mean CE`` into the flat buffer; returns the mean CE.
+                         accumulate: bool = False, last_micro: bool = True, grad_scale: float = 1.0,
+                         teacher: Teacher | None = None) -> torch.Tensor:
+        """Accumulates gradients of ``loss_scale * mean CE`` into the flat buffer; returns the mean CE. With a
+        ``teacher`` (``ids`` and ``logits`` [B, T, K]) the loss is the mean of
+        ``alpha t^2 KL(teacher || student) + (1 - alpha) CE`` (:mod:`bitresearch_b200.ops.distill`).
 
         On the last micro-batch of a step the bucket hook fires as each bucket's gradients become
         final (``grad_scale`` is the loss scale to divide out when packing them)."""
@@ -284,9 +326,12 @@ class FusedGPTEngine:
                     for g in self.grads.values():
                         g.zero_()
             b["loss"].zero_()
-            self._head(tg, b, loss_scale / (B * self.T), grad=True)
+            if teacher is None:
+                self._head(tg, b, loss_scale / (B * self.T), grad=True)
+            else:
+                self._teacher_head(tg, b, loss_scale / (B * self.T), teacher)
         with traced(self.timer, "backward"):  # includes the bucket hooks that launch the gradient reduce
-            self._backward(idx, tg, b, B)
+            self._backward(idx, tg, b, B, scaled=teacher is None)
         return b["loss"][0] / loss_scale
 
     @torch.no_grad()

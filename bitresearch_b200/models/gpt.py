@@ -61,6 +61,8 @@ class GPT(nn.Module):
         self.init_weights(init, seed)
         self.compute_dtype: torch.dtype | None = None  # matmul operand dtype of the eager path
         self.attn_impl = "sdpa"  # eager attention: "sdpa" or "flex" (fused sliding window, under torch.compile)
+        # a token id that starts a document: attention then stays inside documents; None: rows are one sequence
+        self.document_bos: int | None = None
         cos, sin = _rope(cfg.sequence_len, cfg.head_dim, device)
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
@@ -134,6 +136,7 @@ class GPT(nn.Module):
                 return a @ w
             return (a.to(cd) @ w.to(cd)).float()
 
+        docs = None if self.document_bos is None else (idx == self.document_bos).cumsum(1)  # [B, T] document numbers
         x = _rms(P["wte"][idx])
         x0 = x
         cur = x
@@ -151,7 +154,7 @@ class GPT(nn.Module):
                 v = v + P[f"ve_{i}"][idx].view(B, T, KV, hd) * gate
             q = _rms(_rotary(q, cos, sin))
             k = _rms(_rotary(k, cos, sin))
-            o = _attention(q, k, v, effective_window(self.window_sizes[i][0], T), cd, self.attn_impl)
+            o = _attention(q, k, v, effective_window(self.window_sizes[i][0], T), cd, self.attn_impl, docs)
             cur = cur + mm(o.reshape(B * T, D), P[f"layer{i}_proj"]).view(B, T, D)
             h = F.relu(mm(_rms(cur).reshape(B * T, D), P[f"layer{i}_fc"])).square()
             cur = cur + mm(h, P[f"layer{i}_mlp_proj"]).view(B, T, D)
@@ -207,12 +210,15 @@ def _flex_attention(q, k, v, window: int):
     return flex_attention(q, k, v, block_mask=_FLEX_MASKS[key], enable_gqa=k.shape[1] != q.shape[1])
 
 
-def _attention(q, k, v, window: int, cd, impl: str = "sdpa"):
+def _attention(q, k, v, window: int, cd, impl: str = "sdpa", docs=None):
     """q,k,v [B,T,H|KV,hd]; causal with a ``window``-key band (keys i-window+1..i). ``impl='flex'`` runs
-    flex attention (meant to be used under ``torch.compile``) instead of SDPA with a boolean band mask."""
+    flex attention (meant to be used under ``torch.compile``) instead of SDPA with a boolean band mask. ``docs``
+    [B, T]: keys of another document number are not seen."""
     B, T, H, hd = q.shape
     KV = k.shape[2]
     if impl == "flex":
+        if docs is not None:
+            raise ValueError("attention inside documents runs with attn_impl='sdpa'")
         q, k, v = (t.transpose(1, 2) for t in (q, k, v))
         if cd is not None:
             q, k, v = q.to(cd), k.to(cd), v.to(cd)
@@ -223,11 +229,13 @@ def _attention(q, k, v, window: int, cd, impl: str = "sdpa"):
     q, k, v = (t.transpose(1, 2) for t in (q, k, v))
     if cd is not None:
         q, k, v = q.to(cd), k.to(cd), v.to(cd)
-    if window >= T:
+    if window >= T and docs is None:
         o = F.scaled_dot_product_attention(q, k, v, is_causal=True)
     else:
         i = torch.arange(T, device=q.device).view(T, 1)
         j = torch.arange(T, device=q.device).view(1, T)
         mask = (j <= i) & (j > i - window)
+        if docs is not None:
+            mask = (mask & (docs[:, :, None] == docs[:, None, :])).unsqueeze(1)
         o = F.scaled_dot_product_attention(q, k, v, attn_mask=mask)
     return o.float().transpose(1, 2)

@@ -1,9 +1,21 @@
 """The loss against a teacher's top logits, with its gradient."""
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from ._ext import ext
+
+
+@dataclass
+class Teacher:
+    """A teacher's top entries for the tokens of a micro-batch, and how they enter the loss."""
+
+    ids: torch.Tensor  # int32 [..., K], -1: an unused place
+    logits: torch.Tensor  # [..., K]
+    temperature: float = 1.0
+    alpha: float = 1.0  # weight of the teacher's part; the hard labels have 1 - alpha
 
 
 def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,

@@ -38,7 +38,7 @@ import torch.distributed as dist
 from . import checkpoint as ckpt
 from .config import TrainConfig, apply_overrides, estimate_params, preset
 from .data.pipeline import PinnedPrefetcher, make_batch_source
-from .data.synthetic import make_token_bytes
+from .data.synthetic import bos_id, make_token_bytes
 from .data.loader import discover_token_bytes, load_token_bytes
 from .eval import evaluate_bpb
 from .models.gpt import GPT
@@ -132,6 +132,12 @@ class Trainer:
         cfg = self.cfg
         torch.manual_seed(cfg.seed)
         self.model = GPT(cfg.model, init="karpathy", seed=42, device=self.device)
+        if cfg.document_mask:
+            if cfg.torch_compile and cfg.impl == "torch":
+                raise ValueError("document_mask=true does not run with torch_compile=true (flex attention)")
+            if cfg.data == "tokens" and cfg.bos_token_id < 0:
+                raise ValueError("document_mask=true with data=tokens needs bos_token_id, the tokenizer's BOS id")
+            self.model.document_bos = cfg.bos_token_id if cfg.bos_token_id >= 0 else bos_id(cfg.model.vocab_size)
         self._fwd = self.model.forward_torch
         if cfg.torch_compile and cfg.impl == "torch" and self.is_cuda:
             self.model.attn_impl = "flex"
