@@ -210,16 +210,16 @@ __device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool w
 // would share. Items go from the last rows to the first: in a long sequence the late rows cost most.
 //   warp 0     takes items, hands them to the other warps through a two-slot ring, and loads K and V tiles (TMA) into
 //              rings;
-//   warp 1     issues the MMAs, by blocks of 64 keys with two score sets (set s = t % 2). Per query tile X: S_X = Q_X K_t^T
+//   warps 1, 2 issue the MMAs of tile A and of B, by blocks of 64 keys with two score sets (set s = t % 2): S_X = Q_X K_t^T
 //              -> TMEM [256X + 64s, +64) fp32; P_X, written there by the softmax warps as 16-bit pairs over S_X, is
 //              the A operand of O_X += P_X V_t -> TMEM [256X + 128, +D). Order: PV_X(t), S_X(t+2), so the scores of
-//              block t + 1 stand ready while t's softmax runs, and neither waits for the other;
+//              block t + 1 stand ready while t's softmax runs, and neither waits for the other. One thread for both
+//              tiles took 600 to 1000 cycles for a block's twelve MMAs, its waits and commits, twice what they run;
 //   warp 3     loads the Q tiles, one lane each;
 //   warps 4-11 softmax, one query row per thread (4-7 tile A, 8-11 tile B), and the output through shared memory.
-// The two tiles meet only in the K and V rings (a slot is free when both have passed it) and the issuing thread
-// takes whichever is ready, so one may be in its next item while the other finishes: with short sequences an
-// item is few blocks, and what it costs to start and to end one (loads, output) hides behind the other tile's
-// work.
+// The two tiles meet only in the K and V rings (a slot is free when both have passed it), so one may be in its next
+// item while the other finishes: with short sequences an item is few blocks, and what it costs to start and
+// to end one (loads, output) hides behind the other tile's work.
 // P is at most 2^8 (the running maximum is only replaced when it grows by more than that) and is rounded to 16
 // bits for the product (half a step, relative); the row sum l adds the unrounded fp32 values, the maximum, l and
 // O stay in fp32.
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
   uint64_t* o_empty = bars + 14;    // [2]
   uint64_t* item_full = bars + 16;  // [2] ring slots
   uint64_t* item_empty = bars + 18;
-  uint64_t* drain = bars + 20;
+  uint64_t* drain = bars + 50;      // [2]
   uint64_t* clc_full = bars + 21;
   uint64_t* k_full = bars + 22;
   uint64_t* k_empty = k_full + C::kK;
@@ -368,7 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
       mbar_init(&item_full[x], 1);
       mbar_init(&item_empty[x], 12);  // the MMA thread for each tile, two Q loaders, one lane of each softmax warp
     }
-    mbar_init(drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     mbar_init(clc_full, 1);
     for (int i = 0; i < C::kK; ++i) {
       mbar_init(&k_full[i], 1);
@@ -474,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
         if (nc > 0) mbar_wait(clc_full, (nc - 1) & 1, kDrainNs, nullptr);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp < 3) {
     if (elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc_16<T>(BT, BB, false, false);
       constexpr uint32_t idesc_o = umma_idesc_16<T>(BT, D, false, true);
@@ -488,13 +489,11 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
         bool open, pv;   // in an item; the product with V_t (or its passing) is done
         bool end;
       };
-      Place pl[2] = {};
+      Place w = {};
+      const int x = warp - 1;
+      const uint32_t tm = tmem + x * 256;
       // the tile's next product, if what it needs is there; true if something was done
-      auto step = [&](auto xc) {
-        constexpr int x = decltype(xc)::value;
-        Place& w = pl[x];
-        const uint32_t tm = tmem + x * 256;
-        if (w.end) return false;
+      auto step = [&]() {
         if (!w.open) {
           const int slot = w.n & 1;
           if (!mbar_test(&item_full[slot], (w.n >> 1) & 1)) return false;
@@ -504,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
           }
           const FwdItem I = item_of(slot);
           mbar_arrive(&item_empty[slot]);
-          w.t0 = I.first(), w.t1 = I.last(), w.lo = I.lo[x], w.hi = I.hi[x];
+          w.t0 = I.first(), w.t1 = I.last(), w.lo = x ? I.lo[1] : I.lo[0], w.hi = x ? I.hi[1] : I.hi[0];
           w.t = w.t0 - 2;
           w.open = true;
           w.pv = false;
@@ -565,9 +564,8 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
       };
       uint64_t since = globaltimer_ns();
       bool ok = true;
-      for (uint32_t spin = 0; !(pl[0].end && pl[1].end);) {
-        const bool a = step(std::integral_constant<int, 0>{}), b = step(std::integral_constant<int, 1>{});
-        if (a || b) {
+      for (uint32_t spin = 0; !w.end;) {
+        if (step()) {
           spin = 0;
         } else if ((++spin & 255u) == 0) {
           if (spin == 256) since = globaltimer_ns();
@@ -579,10 +577,9 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
         }
       }
       if (!ok) fail(kErrTimeoutMma);
-      umma_commit(drain);
-      mbar_wait(drain, 0, kDrainNs, nullptr);
+      umma_commit(&drain[x]);
+      mbar_wait(&drain[x], 0, kDrainNs, nullptr);
     }
-  } else if (warp == 2) {
   } else if (warp == 3) {
     const int x = lane_id();
     if (x < 2) {
