@@ -165,6 +165,20 @@ def test_strides_alignment_and_place(cuda, V, dt):
     assert none is None and torch.equal(r3, rows)
 
 
+def test_offsets_past_32_bits(cuda):
+    op, _ = _op()
+    M, V, K = 34_000, 65_536, 4
+    if torch.cuda.get_device_properties(0).total_memory < 30e9:
+        pytest.skip("needs 30 GB")
+    z = torch.empty(M, V, dtype=torch.bfloat16, device="cuda").normal_(std=3.0)
+    ids = torch.randint(0, V, (M, K), device="cuda", dtype=torch.int32)
+    u = torch.randn(M, K, device="cuda")
+    last = z[-2:].clone()
+    _, rows, _ = op(z, ids, u, cap=15.0, scale=1.0, grad=z)
+    r, g, rt, gt = reference(last, ids[-2:], u[-2:], None, 15.0, 1.0, 1.0, 1.0)
+    assert ((rows[-2:].double().cpu() - r).abs() <= rt).all() and ((z[-2:].double().cpu() - g).abs() <= gt).all()
+
+
 def test_empty_batch_and_default_scale(cuda):
     op, _ = _op()
     z, ids, u, y = _inputs(4, 100, 8, torch.bfloat16, 15.0)

@@ -179,6 +179,29 @@ def test_bad_spans_stay_inside(cuda):
     assert check_status() == 0
 
 
+def test_offsets_past_32_bits(cuda):
+    """2.4e9 elements of q: the last sequences' results are those of the same rows alone."""
+    packed, check_status = _ops()
+    n, H, D, length = 300_007, 64, 128, 500
+    if torch.cuda.get_device_properties(0).total_memory < 60e9:
+        pytest.skip("needs 60 GB")
+    lengths = [length] * (n // length) + [n % length]
+    off = torch.tensor([0] + lengths).cumsum(0).to(torch.int32).cuda()
+    start, end = packed.bounds_from_offsets(off, n)
+    q = torch.randn(n, H, D, device="cuda", dtype=torch.bfloat16)
+    k, v = (torch.randn(n, 1, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    out, lse = packed.attention_fwd(q, k, v, start, end)
+    dq, dk, dv = packed.attention_bwd(q, k, v, out, lse, q, start, end)
+    torch.cuda.synchronize()
+    assert check_status() == 0
+    a = n - 7 - 3 * length  # whole tiles lie elsewhere in the slice, so sums are added in another order
+    s, e = (t[a:] - a for t in (start, end))
+    ref = attention(q[a:], k[a:], v[a:], s, e, 0, 1 / math.sqrt(D), q[a:])
+    for name, got in dict(out=out, dq=dq, dk=dk, dv=dv).items():
+        _within(got[a:], ref[name], name)
+    _within(lse[:, a:], ref["lse"], "lse")
+
+
 def test_empty(cuda):
     packed, _ = _ops()
     q, k, v = _make(0, 2, 1, 64, torch.bfloat16, "plain")
