@@ -889,9 +889,13 @@ __device__ __forceinline__ bool store_cols(uint32_t taddr, float f, const Rows& 
   return odd != 0.f;
 }
 
-// dQ. TMEM: two score sets (set s, for the blocks of group s: S at [128s, +64), dP at [128s + 64, +64)); dQ at [256, +D); the block's Q and dO rows as 16-bit pairs at [384, +D/2)
-// and [448, +D/2): the S and dP products read only K and V from shared memory. The kernel also computes
-// delta = rowsum(dO o O) and leaves (lse, delta) of each row for the dK/dV kernel.
+// dQ. TMEM: two score sets (set s, for the blocks of group s: S at [128s, +64), dP at [128s + 64, +64)); dQ at
+// [256, +D); the tile's Q and dO rows as 16-bit pairs at [384, +D/2) and [448, +D/2): the S and dP products read only
+// K and V from shared memory. The kernel also computes delta = rowsum(dO o O) and leaves lse and delta of each row
+// for the dK/dV kernel. Two roundings are undone here, since with dS rounded once and O's rounding in delta, dQ
+// and dK came out 1.5 to 1.6 times as far from 64 bits as one rounding of the result alone: dQ takes dS in two
+// 16-bit parts (a third more products), and the delta that goes to dK/dV is the sum of P dP itself, in fp32, which
+// this kernel has at hand.
 template <int D>
 struct DqCfg {
   static constexpr int kTile = BB * D * 2;
@@ -899,8 +903,8 @@ struct DqCfg {
   static constexpr int oK = 0, oV = kStages * kTile;
   // the tile's Q and dO rows wait in the ring's stages 3 and 4 until they are in TMEM, its O rows by themselves
   static constexpr int oQ = oK + 3 * kTile, oD = oV + 3 * kTile, oO = oV + kStages * kTile;
-  static constexpr int oSum = oO + 2 * kTile;  // [2][128] half-row sums
-  static constexpr int oBar = oSum + 1024;
+  static constexpr int oSum = oO + 2 * kTile;  // [2][128] half-row sums, [128] one group's share of delta
+  static constexpr int oBar = oSum + 1536;
   static constexpr int kSmem = oBar + 256 + 1024;
   static_assert(kSmem <= 232448, "dQ shared memory");
 };
@@ -926,7 +930,8 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
   uint64_t* kv_empty = kv_full + C::kStages;
   uint64_t* in_full = kv_empty + C::kStages;  // Q, dO and O have arrived
   uint64_t* in_read = in_full + 1;            // Q and dO are in TMEM
-  static_assert(8 + 2 * C::kStages <= 28, "barrier region");
+  uint64_t* sums_full = in_read + 1;          // both groups' shares of delta stand in shared memory
+  static_assert(9 + 2 * C::kStages <= 28, "barrier region");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -942,6 +947,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     mbar_init(q_full, 256);  // every softmax thread has stored its Q or dO row in TMEM
     mbar_init(in_full, 1);
     mbar_init(in_read, 256);
+    mbar_init(sums_full, 256);
     mbar_init(done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -1023,8 +1029,8 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         const int st = j % C::kStages;
         const uint64_t k_desc = mn_major(smem + C::oK + st * C::kTile, kAtom64);
 #pragma unroll
-        for (int kk = 0; kk < BB / 16; ++kk)  // dS as 16-bit pairs at the first 32 columns of its set
-          umma_bf16_ts(tmem + 256, tmem + (j & 1) * 128 + kk * 8, k_desc + kk * (2048 >> 4), idesc_q,
+        for (int kk = 0; kk < BB / 8; ++kk)  // dS and what its rounding left, 16-bit pairs at columns 0 and 32 of the set
+          umma_bf16_ts(tmem + 256, tmem + (j & 1) * 128 + kk * 8, k_desc + kk % (BB / 16) * (2048 >> 4), idesc_q,
                        (j > 0 || kk > 0) ? 1u : 0u);
         umma_commit(&kv_empty[st]);
         if (j + 2 < nb) ok = issue_s(j + 2);  // into the set that this product has read
@@ -1085,10 +1091,10 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       sums[half * 128 + r] = acc;
       asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps
       stat = make_float2(lse, real ? sums[r] + sums[128 + r] : 0.f);
-      if (half == 0) p.stat[(int64_t)h * p.Np + i] = make_float2(-stat.x, -stat.y);
     }
     const int z = __ldg(p.start + q0);  // keys before it are foreign to every row of the tile: all in block kb_lo
     const uint32_t set_base = lane_base + half * 128;
+    uint64_t exact = 0;  // sum of P dP: delta without the rounding of O
     for (int j = half; ok && j < nb; j += 2) {
       if (!mbar_wait_warp(&s_full[half], (j >> 1) & 1, kBudgetNs, abort_flag, status)) {
         fail(kErrTimeoutEpilogue);
@@ -1097,7 +1103,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       }
       tc_fence_after();
       const int k0 = (kb_lo + j) * BB;
-      uint32_t pk[32];
+      uint32_t pk[32], rest[32];
       // dS = P (dP - delta), 0 where the row does not see the key
       uint32_t svs[2][32], dvs[2][32];
 #pragma unroll
@@ -1116,13 +1122,22 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float2 y = f32x2_split(fma_f32x2(f32x2(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), sc2, nl2));
-          float2 g = f32x2_split(mul_f32x2(f32x2(exp2f(y.x), exp2f(y.y)),
-                                           sub_f32x2(f32x2(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), dl2)));
+          const uint64_t pr = f32x2(exp2f(y.x), exp2f(y.y));
+          const uint64_t dp = f32x2(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1]));
+          float2 g = f32x2_split(mul_f32x2(pr, sub_f32x2(dp, dl2)));
           if constexpr (kMasked) {
-            g.x = ((vis >> e) & 1u) ? g.x : 0.f;
-            g.y = ((vis >> (e + 1)) & 1u) ? g.y : 0.f;
+            const bool v0 = (vis >> e) & 1u, v1 = (vis >> (e + 1)) & 1u;
+            g.x = v0 ? g.x : 0.f;
+            g.y = v1 ? g.y : 0.f;
+            const float2 t = f32x2_split(mul_f32x2(pr, dp));
+            exact = add_f32x2(exact, f32x2(v0 ? t.x : 0.f, v1 ? t.y : 0.f));
+          } else {
+            exact = fma_f32x2(pr, dp, exact);
           }
-          pk[c * 16 + e / 2] = Half16<T>::pack(g.x, g.y);
+          const uint32_t hi = Half16<T>::pack(g.x, g.y);
+          const float2 back = Half16<T>::unpack(hi);
+          pk[c * 16 + e / 2] = hi;
+          rest[c * 16 + e / 2] = Half16<T>::pack(g.x - back.x, g.y - back.y);
         }
       };
       if (__all_sync(0xffffffffu, key.x <= k0 && key.y >= k0 + BB)) {
@@ -1140,9 +1155,22 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       }
       __syncwarp();
       tmem_st32(set_base, pk);
+      tmem_st32(set_base + 32, rest);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_full[half]);
+    }
+    // delta for the dK/dV kernel
+    {
+      float* sums = reinterpret_cast<float*>(smem + C::oSum);
+      const float2 e2 = f32x2_split(exact);
+      const float mine = e2.x + e2.y;
+      if (half == 1) sums[256 + r] = mine;
+      mbar_arrive(sums_full);
+      if (half == 0) {
+        ok = mbar_wait_warp(sums_full, 0, kBudgetNs, abort_flag, status) && ok;
+        p.stat[(int64_t)h * p.Np + i] = make_float2(-stat.x, real ? -(mine + sums[256 + r]) : 0.f);
+      }
     }
     if (ok && mbar_wait_warp(done, 0, kBudgetNs, abort_flag, status)) {
       tc_fence_after();
