@@ -893,9 +893,10 @@ __device__ __forceinline__ bool store_cols(uint32_t taddr, float f, const Rows& 
 // [256, +D); the tile's Q and dO rows as 16-bit pairs at [384, +D/2) and [448, +D/2): the S and dP products read only
 // K and V from shared memory. The kernel also computes delta = rowsum(dO o O) and leaves lse and delta of each row
 // for the dK/dV kernel. Two roundings are undone here, since with dS rounded once and O's rounding in delta, dQ
-// and dK came out 1.5 to 1.6 times as far from 64 bits as one rounding of the result alone: dQ takes dS in two
-// 16-bit parts (a third more products), and the delta that goes to dK/dV is the sum of P dP itself, in fp32, which
-// this kernel has at hand.
+// and dK came out 1.5 to 1.6 times as far from 64 bits as one rounding of the result alone: the tile's last two
+// blocks, where the rows of few keys and large weights have all of theirs, take dS in two 16-bit parts, and the
+// delta that goes to dK/dV is the sum of P dP itself, in fp32, which this kernel has at hand. (Both parts in every
+// block: 219 instead of 184 us over 65536 packed tokens.)
 template <int D>
 struct DqCfg {
   static constexpr int kTile = BB * D * 2;
@@ -1029,9 +1030,14 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         const int st = j % C::kStages;
         const uint64_t k_desc = mn_major(smem + C::oK + st * C::kTile, kAtom64);
 #pragma unroll
-        for (int kk = 0; kk < BB / 8; ++kk)  // dS and what its rounding left, 16-bit pairs at columns 0 and 32 of the set
-          umma_bf16_ts(tmem + 256, tmem + (j & 1) * 128 + kk * 8, k_desc + kk % (BB / 16) * (2048 >> 4), idesc_q,
+        for (int kk = 0; kk < BB / 16; ++kk)  // dS as 16-bit pairs at the first 32 columns of its set
+          umma_bf16_ts(tmem + 256, tmem + (j & 1) * 128 + kk * 8, k_desc + kk * (2048 >> 4), idesc_q,
                        (j > 0 || kk > 0) ? 1u : 0u);
+        if (j >= nb - 2) {
+#pragma unroll
+          for (int kk = 0; kk < BB / 16; ++kk)  // and what its rounding left, in the next 32
+            umma_bf16_ts(tmem + 256, tmem + (j & 1) * 128 + 32 + kk * 8, k_desc + kk * (2048 >> 4), idesc_q, 1u);
+        }
         umma_commit(&kv_empty[st]);
         if (j + 2 < nb) ok = issue_s(j + 2);  // into the set that this product has read
       }
@@ -1112,8 +1118,8 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         tmem_ld32(set_base + 64 + c * 32, dvs[c]);
       }
       tmem_ld_wait();
-      auto body = [&](int c, auto masked) {
-        constexpr bool kMasked = decltype(masked)::value;
+      auto body = [&](int c, auto masked, auto split) {
+        constexpr bool kMasked = decltype(masked)::value, kSplit = decltype(split)::value;
         const uint32_t(&sv)[32] = svs[c];
         const uint32_t(&dv)[32] = dvs[c];
         uint32_t vis = 0xffffffffu;
@@ -1135,17 +1141,23 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
             exact = fma_f32x2(pr, dp, exact);
           }
           const uint32_t hi = Half16<T>::pack(g.x, g.y);
-          const float2 back = Half16<T>::unpack(hi);
           pk[c * 16 + e / 2] = hi;
-          rest[c * 16 + e / 2] = Half16<T>::pack(g.x - back.x, g.y - back.y);
+          if constexpr (kSplit) {
+            const float2 back = Half16<T>::unpack(hi);
+            rest[c * 16 + e / 2] = Half16<T>::pack(g.x - back.x, g.y - back.y);
+          }
         }
       };
-      if (__all_sync(0xffffffffu, key.x <= k0 && key.y >= k0 + BB)) {
-        body(0, std::false_type{});
-        body(1, std::false_type{});
+      const bool split = j >= nb - 2;
+      if (split) {
+        body(0, std::true_type{}, std::true_type{});
+        body(1, std::true_type{}, std::true_type{});
+      } else if (__all_sync(0xffffffffu, key.x <= k0 && key.y >= k0 + BB)) {
+        body(0, std::false_type{}, std::false_type{});
+        body(1, std::false_type{}, std::false_type{});
       } else {
-        body(0, std::true_type{});
-        body(1, std::true_type{});
+        body(0, std::true_type{}, std::false_type{});
+        body(1, std::true_type{}, std::false_type{});
       }
       if (j == 0 && r < BB && kb_lo * BB + r < z) {
         uint4* row = reinterpret_cast<uint4*>(smem + C::oK + r * 128);
@@ -1155,7 +1167,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       }
       __syncwarp();
       tmem_st32(set_base, pk);
-      tmem_st32(set_base + 32, rest);
+      if (split) tmem_st32(set_base + 32, rest);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_full[half]);
