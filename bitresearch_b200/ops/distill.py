@@ -35,7 +35,8 @@ def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     ``alpha < 1``. Any other id outside ``[0, V)`` is skipped and reported through the device status word.
 
     ``grad`` may be given, also as ``logits`` itself (in place). ``need_grad=False`` returns the loss alone. Runs on
-    the current stream of the logits' device; the same inputs give the same bits. Wrong arguments raise
+    the current stream of the logits' device, in a captured graph too (once any kernel of this package has run on
+    that device); the same inputs give the same bits. Wrong arguments raise
     ``ValueError``."""
     if scale is None:
         scale = 1.0 / max(1, logits.shape[0])

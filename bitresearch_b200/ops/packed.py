@@ -11,7 +11,8 @@ padding rows hold; rows of no sequence are left as they were in every output (ze
 Spans must be those of sequences that follow one another; any other contents give wrong values but read and
 write no row outside the tensors.
 
-Calls run on the current stream of the tensors' device, in a captured graph too, allocate only the outputs and the
+Calls run on the current stream of the tensors' device, in a captured graph too (once any kernel of this package
+has run on that device), allocate only the outputs and the
 backward's scratch when they are not given, and give the same bits for the same inputs. Wrong arguments raise ``ValueError``.
 """
 from __future__ import annotations
