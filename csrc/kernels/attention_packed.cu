@@ -11,7 +11,7 @@
 // Key row j is seen by the queries [j, min(j + w, end[j])). Rows of no sequence (empty span) are neither read
 // as keys nor written. Spans are clamped to the rows that exist, so a bad span reads nothing outside.
 //
-// Forward: tcgen05 tiles of 128 packed rows by 128 packed keys (described at the kernel). A tile may hold the end of
+// Forward: tcgen05 tiles of 128 packed rows by 64 packed keys (described at the kernel). A tile may hold the end of
 // one sequence and the start of the next: the tiles are cut by row number, not by sequence, so a batch of
 // short sequences fills them as well as one long sequence does, no work list has to be built, and the sequences
 // appear only as each row's range of keys. A matrix product multiplies hidden keys by a weight of exactly 0,
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
     if (elect_one()) {
       tma_prefetch_desc(&maps.k);
       tma_prefetch_desc(&maps.v);
-      int ik = 0, iv = 0, nc = 0;  // K and V tiles loaded so far (ring positions), requests for work
+      int ik = 0, iv = 0, nc = 0;  // K and V blocks loaded so far (ring positions), requests for work
       bool ok = true;
       auto publish = [&](int n, int block, FwdItem& I) {
         volatile int* slot = ring + (n & 1) * 4;
