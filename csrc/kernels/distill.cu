@@ -149,9 +149,12 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
   constexpr bool kTwoSums = MODE == kSquare || MODE == kHard;
   extern __shared__ __align__(16) uint8_t smem[];  // [S][kPiece] vectors; per entries' warp q, l, id [K] and a hash table
   __shared__ uint64_t full[S], empty[S], written[TW];
-  __shared__ float red[2][2][kWarps], redm[2][kWarps];  // by parity of the row
-  __shared__ float2 part[2], partm[2];                  // this block's sums and maximum, read by the cluster's others
-  __shared__ float s_m[2];
+  // A row's sums and maximum, read by the holding warps and by the row's entries' warp after both(n). That warp may still
+  // read them while the holding warps go on as far as row n + TW, whose both() it has to reach first: TW + 1 places.
+  constexpr int kPlaces = TW + 1;
+  __shared__ float red[kPlaces][2][kWarps], s_m[kPlaces];
+  __shared__ float redm[2][kWarps];     // by parity of the row: only the holding warps', which meet twice in between
+  __shared__ float2 part[2], partm[2];  // this block's sums and maximum, read by the cluster's others
   __shared__ struct { int some, y; float ly; } info[TW];
   asm volatile("griddepcontrol.launch_dependents;");
   const int cs = p.cluster, rank = cs > 1 ? (int)cluster_rank() : 0;
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
   if (warp < kWarps) {
     int n = 0;
     for (int64_t row = first; row < p.M; row += stride, ++n) {
-      const int par = n & 1;
+      const int par = n & 1, place = n % kPlaces;
       const Row r = row_of(row);
       // edge elements: one for each of the first threads of the row's first block
       const bool has_edge = rank == 0 && tid < r.n_head + p.V - r.tail;
@@ -304,7 +307,7 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
         }
         if (m == -INFINITY) m = 0.f;  // nothing to take them relative to
         again();
-        if (tid == 0) s_m[par] = m;
+        if (tid == 0) s_m[place] = m;
       }
       uint64_t st2 = soft(edge, -INFINITY, m), s12 = 0;
       if constexpr (kTwoSums) s12 = hard(edge, -INFINITY, m, st2);
@@ -324,12 +327,12 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
       {
         const float2 a = f32x2_split(st2), b = f32x2_split(s12);
         const float st = warp_sum(a.x + a.y), s1 = kTwoSums ? warp_sum(b.x + b.y) : 0.f;
-        if (lane == 0) red[par][0][warp] = st, red[par][1][warp] = s1;
+        if (lane == 0) red[place][0][warp] = st, red[place][1][warp] = s1;
       }
       both(n);
       float2 sums = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) sums = make_float2(sums.x + red[par][0][w], sums.y + red[par][1][w]);
+      for (int w = 0; w < kWarps; ++w) sums = make_float2(sums.x + red[place][0][w], sums.y + red[place][1][w]);
       if (cs > 1) {
         if (tid == 0) part[par] = sums;
         sums = meet(false, par, sums);
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
     };
     int n = 0;
     for (int64_t row = first; row < p.M; row += stride, ++n) {
-      const int par = n & 1;
+      const int par = n & 1, place = n % kPlaces;
       if (n % TW != turn) {
         if (cs > 1) {  // every thread of the cluster meets
           if (need_max) meet(true, par, make_float2(0.f, 0.f));
@@ -475,9 +478,9 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
       if (need_max && cs > 1) meet(true, par, make_float2(0.f, 0.f));
       both(n);
       float2 sums = make_float2(0.f, 0.f);
-      for (int w = 0; w < kWarps; ++w) sums = make_float2(sums.x + red[par][0][w], sums.y + red[par][1][w]);
+      for (int w = 0; w < kWarps; ++w) sums = make_float2(sums.x + red[place][0][w], sums.y + red[place][1][w]);
       if (cs > 1) sums = meet(false, par, sums);
-      const float m = need_max ? s_m[par] : p.cap;
+      const float m = need_max ? s_m[place] : p.cap;
       const Factors f = factors(m, sums, some, y, ly);
       if (lane == 0 && rank == 0) {
         float loss = f.loss;
