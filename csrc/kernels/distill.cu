@@ -156,6 +156,8 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
   __shared__ float redm[2][kWarps];     // by parity of the row: only the holding warps', which meet twice in between
   __shared__ float2 part[2], partm[2];  // this block's sums and maximum, read by the cluster's others
   __shared__ struct { int some, y; float ly; } info[TW];
+  __shared__ int s_gave_up;
+  volatile int* gave_up = &s_gave_up;
   asm volatile("griddepcontrol.launch_dependents;");
   const int cs = p.cluster, rank = cs > 1 ? (int)cluster_rank() : 0;
   const int64_t first = blockIdx.x / cs, stride = gridDim.x / cs;
@@ -166,13 +168,18 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
       mbar_init(&empty[i], kWarps);
     }
     for (int i = 0; i < TW; ++i) mbar_init(&written[i], kWarps);
+    s_gave_up = 0;
     fence_barrier_init();
   }
   __syncthreads();
-  // A wait that runs out records it and goes on, so that every thread still meets every barrier; after the first
-  // failure on the device no further wait spends its budget.
+  // A wait that runs out records it and its thread goes on, so that every thread still meets every barrier; no further
+  // wait of the block spends its budget then. The device's status word ends no wait: it may hold a bad id, of this
+  // launch's own rows among others, and all rows but that one are to come out right.
   auto wait = [&](uint64_t* bar, int64_t phase) {
-    if (!mbar_wait(bar, phase & 1, kBudgetNs, nullptr, p.status)) atomicCAS(p.status, 0, (int)kErrTimeoutProducer);
+    if (mbar_wait(bar, phase & 1, kBudgetNs, gave_up)) return true;
+    *gave_up = 1;
+    atomicCAS(p.status, 0, (int)kErrTimeoutProducer);
+    return false;
   };
   // a row: edge elements before its first 16-byte boundary, nvec whole vectors, edge elements behind them
   struct Row {
@@ -494,8 +501,10 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
       }
     }
   } else {
-    // the producer: this block's whole vectors of each row, S rows ahead
+    // the producer: this block's whole vectors of each row, S rows ahead; none any more once a wait has run out
+    int issued = 0;
     auto load = [&](int64_t row, int n) {
+      issued = n + 1;
       const Row r = row_of(row);
       const int count = max(0, min(r.nvec - rank * kPiece, kPiece));
       mbar_arrive_expect_tx(&full[n % S], count * 16);
@@ -511,12 +520,13 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
         if (need_max) cluster_sync_all();
         cluster_sync_all();
       }
-      if (lane == 0 && row + S * stride < p.M) {
-        wait(&empty[n % S], n / S);
-        load(row + S * stride, n + S);
-      }
+      if (lane == 0 && row + S * stride < p.M && !*gave_up && wait(&empty[n % S], n / S)) load(row + S * stride, n + S);
       __syncwarp();
     }
+    // the block's shared memory stays until the last copies have landed
+    if (lane == 0)
+      for (int n = max(0, issued - S); n < issued; ++n) mbar_wait(&full[n % S], (n / S) & 1, kBudgetNs, nullptr);
+    __syncwarp();
   }
   if (cs > 1) cluster_sync_all();  // the others may still read this block's sums
 }

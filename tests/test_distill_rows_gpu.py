@@ -113,3 +113,19 @@ def test_short_rows_in_turn(cuda):
         assert torch.equal(rows, first)
         assert grad is None or ((grad.double() - g).abs() <= gt).all()
     assert ((first.double() - r).abs() <= rt).all()
+
+
+@pytest.mark.parametrize("M,V,dt", [FORMS[1], FORMS[4], FORMS[6], FORMS[7]], ids=lambda x: str(x).replace("torch.", ""))
+@pytest.mark.parametrize("t,alpha", [(1.0, 1.0), (2.0, 0.5)])
+def test_a_bad_id_costs_its_own_entry_alone(cuda, M, V, dt, t, alpha):
+    """Ids outside the vocabulary in the first rows, while thousands of waits of the other rows are still to come; and a
+    call while the status word still holds the last one's report."""
+    op, check_status = _op()
+    z, ids, u, y = inputs(M, V, 16, dt, 15.0, seed=V + 1)
+    ids[0, 3], ids[1, 0], ids[2] = V, -7, 2 ** 31 - 1
+    y[3] = V
+    r, g, rt, gt = reference(z, ids, u, y, 15.0, t, alpha, 1.0)
+    for _ in range(2):
+        _, rows, grad = op(z, ids, u, y, cap=15.0, temperature=t, alpha=alpha, scale=1.0)
+        assert ((rows.double() - r).abs() <= rt).all() and ((grad.double() - g).abs() <= gt).all()
+    assert check_status() == BAD_INDEX
