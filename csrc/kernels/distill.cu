@@ -194,10 +194,14 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
     r.tail = r.n_head + r.nvec * E;
     return r;
   };
-  // with max: the cluster's maximum; else its sums. Every thread of the cluster comes here once per row (and kind)
-  auto meet = [&](bool is_max, int par, float2 s) {
+  // the barrier's instructions want the whole warp at once, and it comes here from branches for one lane
+  auto cluster_barrier = [] {
     __syncwarp();
     cluster_sync_all();
+  };
+  // with max: the cluster's maximum; else its sums. Every thread of the cluster comes here once per row (and kind)
+  auto meet = [&](bool is_max, int par, float2 s) {
+    cluster_barrier();
     const float2* mine = is_max ? &partm[par] : &part[par];
     s = peer_pair(mine, 0);
     for (int r = 1; r < cs; ++r) {
@@ -517,8 +521,8 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
     int n = 0;
     for (int64_t row = first; row < p.M; row += stride, ++n) {
       if (cs > 1) {
-        if (need_max) cluster_sync_all();
-        cluster_sync_all();
+        if (need_max) cluster_barrier();
+        cluster_barrier();
       }
       if (lane == 0 && row + S * stride < p.M && !*gave_up && wait(&empty[n % S], n / S)) load(row + S * stride, n + S);
       __syncwarp();
@@ -528,7 +532,7 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
       for (int n = max(0, issued - S); n < issued; ++n) mbar_wait(&full[n % S], (n / S) & 1, kBudgetNs, nullptr);
     __syncwarp();
   }
-  if (cs > 1) cluster_sync_all();  // the others may still read this block's sums
+  if (cs > 1) cluster_barrier();  // the others may still read this block's sums
 }
 
 // loss = scale * sum of the rows, in one fixed order: one block, each thread's rows in order in 64 bits. Launched
