@@ -53,8 +53,8 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start: torc
 
 
 def bwd_scratch(rows: int, heads: int) -> int:
-    """Entries of the fp32 scratch of :func:`attention_bwd`: two per head and row, rows rounded up to 128."""
-    return 2 * heads * ((rows + 127) // 128 * 128)
+    """Entries of the fp32 scratch of :func:`attention_bwd`, for both types and any number of kv heads."""
+    return 5 * heads * ((rows + 127) // 128 * 128)  # a row's lse and delta; in fp16 also its factors' three bounds
 
 
 def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,

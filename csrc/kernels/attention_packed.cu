@@ -56,9 +56,31 @@ struct PackedParams {
   const int* start;
   const int* end;
   float* lse;    // [H, N], natural log
-  float2* stat;  // backward scratch [H, Np]: (-lse in log2 units, -delta) of each row; (-inf, 0) for rows of no sequence
+  float2* stat;  // backward scratch [H, Np]: (kUp - lse in log2 units, -delta) of each row; (-inf, 0) for rows of no sequence
+  // fp16 backward scratch, each value the largest of the row's sequence among the 32 rows that hold it
+  float* v_most;   // [KV, Np]: |v|
+  float2* d_most;  // [H, Np]: |do| and |delta|
   int Np;        // N rounded up to whole tiles
 };
+
+// Powers of two that keep the fp16 backward's 16-bit factors in the normal range. P of a long sequence is far below
+// fp16's smallest normal number (2^-14), and dS = P (dP - delta) is as small as the gradients make it; bf16 has fp32's
+// range and needs none of this. P goes to its product times 2^kUp (it is at most 1, but for its fp32 error). dS goes to
+// its product times 2^up_for(b), where b is at least |dP - delta|: below 2^14 P, so normal down to P = 2^-24 where |dP
+// - delta| is b / 16 (dP is a sum of D products, |do| |v| its largest possible value). The factor is undone, exactly,
+// on the fp32 sums. It belongs to a row of the output, so that it follows what that row sees and nothing of other
+// sequences: in dQ b = |do_i| max |v_j| + |delta_i| over the row's keys, in dK/dV b = max |do_i| |v_j| + max |delta_i|
+// over the queries that see the row (and others of its sequence). Rows that are no numbers count as zero there: what
+// sees them is no number anyway.
+template <typename T>
+constexpr bool kScaled = Half16<T>::kFormat == 0;
+template <typename T>
+constexpr float kUp = kScaled<T> ? 14.f : 0.f;
+__device__ __forceinline__ float power_of_2(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ int up_for(float b) {
+  const int e = (__float_as_int(b) >> 23) - 127;  // b < 2^(e + 1)
+  return b > 0.f ? 13 - max(e, -87) : 0;
+}
 
 // ---------------------------------------------------------------------------------------- row by row
 template <typename T, int D>
@@ -199,7 +221,40 @@ __device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool w
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= p.scale;
   }
+  if constexpr (kScaled<T>) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= power_of_2(-(int)kUp<T>);  // stat raised the weights
+  }
   store_row<T, D>(want_dk ? p.dk : p.dv, j, g, lane, acc);
+}
+
+// the largest of the values (none negative) of a warp's lanes that have the same seq
+__device__ __forceinline__ float most_of_seq(float x, int seq) {
+  return __uint_as_float(__reduce_max_sync(__match_any_sync(0xffffffffu, seq), __float_as_uint(x)));
+}
+
+// v_most: one warp per 32 rows of a kv head. It reads V once; before dQ, in fp16 alone.
+constexpr int kNormThreads = 256;
+template <typename T, int D>
+__global__ void __launch_bounds__(kNormThreads) v_most_kernel(const __grid_constant__ PackedParams p) {
+  constexpr int E = D / 32;
+  const int groups = p.Np / 32, lane = lane_id();
+  const int64_t at = (int64_t)blockIdx.x * (kNormThreads / 32) + warp_id();
+  if (at >= (int64_t)groups * p.KV) return;
+  const int g = (int)(at / groups), j0 = (int)(at % groups) * 32, j = j0 + lane;
+  const int first = j < p.N ? __ldg(p.start + j) : 0;
+  const bool real = j < p.N && first <= j && queries_of(p, j) > j;
+  const uint32_t read = __ballot_sync(0xffffffffu, real);  // a row of no sequence is not read
+  float m = 0.f;
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r) {
+    if (!((read >> r) & 1u)) continue;
+    float v[E];
+    load_row<T, D>(p.v, j0 + r, g, lane, v);
+    const float s = dot(v, v);
+    if (lane == r && s < INFINITY) m = sqrtf(s);
+  }
+  p.v_most[(int64_t)g * p.Np + j] = most_of_seq(m, real ? first : -1 - lane);
 }
 
 // ---------------------------------------------------------------------------------------- forward, tcgen05
@@ -1063,6 +1118,17 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     const int2 key = i < p.N ? keys_of(p, i) : make_int2(0, 0);
     const bool real = key.y > key.x;
     const float lse = real ? p.lse[(int64_t)h * p.N + i] * kLog2e : INFINITY;
+    const int seq = real ? __ldg(p.start + i) : -1 - lane;
+    float v_most = 0.f;
+    if constexpr (kScaled<T>) {
+      // the 32 rows with this one among them; before them, rows of one sequence alone are seen: that of their first row
+      const float* most = p.v_most + (int64_t)kvh * p.Np;
+      const int g0 = i - lane, lo = __shfl_sync(0xffffffffu, real ? key.x : g0, 0);
+      float before = 0.f;
+      for (int g = lo / 32 + lane; g < g0 / 32; g += 32) before = fmaxf(before, most[g * 32 + 31]);
+      before = warp_max(before);
+      if (real) v_most = fmaxf(most[i], key.x < g0 ? before : 0.f);
+    }
     bool ok = mbar_wait_warp(in_full, 0, kBudgetNs, abort_flag, status);
     if (!ok) fail(kErrTimeoutEpilogue);
     // 16 bytes, the piece-th of this row of a tile
@@ -1088,9 +1154,11 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     mbar_arrive(q_full);
     // delta: the two warps of a row each reduce half of its values and meet in shared memory
     float2 stat;
+    int up = 0;  // dS goes to its product times 2^up
+    float norm = 0.f;
     {
       float* sums = reinterpret_cast<float*>(smem + C::oSum);
-      float acc = 0.f;
+      float acc = 0.f, norm2 = 0.f;
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) {
         const uint4 a = piece_of(C::oO, half * (D / 16) + e), b = piece_of(C::oD, half * (D / 16) + e);
@@ -1099,13 +1167,26 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         for (int k = 0; k < 4; ++k) {
           const float2 f = Half16<T>::unpack(u[k]), w = Half16<T>::unpack(y[k]);
           acc = fmaf(f.x, w.x, fmaf(f.y, w.y, acc));
+          if constexpr (kScaled<T>) norm2 = fmaf(w.x, w.x, fmaf(w.y, w.y, norm2));
         }
       }
       mbar_arrive(in_read);
       sums[half * 128 + r] = acc;
+      // the halves of |do|^2 meet where each thread has read O: at its first piece
+      auto norm_at = [&](int x) {
+        const int piece = x * (D / 16);
+        return reinterpret_cast<float*>(smem + C::oO + (piece >> 3) * kAtom + r * 128 + (((piece & 7) ^ (r & 7)) << 4));
+      };
+      if constexpr (kScaled<T>) *norm_at(half) = norm2;
       asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps
       stat = make_float2(lse, real ? sums[r] + sums[128 + r] : 0.f);
+      if constexpr (kScaled<T>) {
+        const float n2 = *norm_at(0) + *norm_at(1);
+        norm = real && n2 < INFINITY ? sqrtf(n2) : 0.f;
+        up = up_for(norm * v_most + fabsf(stat.y));
+      }
     }
+    const float from = stat.x - (float)up;  // P times 2^up is exp2(s - from)
     const int z = __ldg(p.start + q0);  // keys before it are foreign to every row of the tile: all in block kb_lo
     const uint32_t set_base = lane_base + half * 128;
     uint64_t exact = 0;  // sum of P dP: delta without the rounding of O
@@ -1132,7 +1213,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         const uint32_t(&dv)[32] = dvs[c];
         uint32_t vis = 0xffffffffu;
         if constexpr (kMasked) vis = range_mask32(key.x - k0 - 32 * c, key.y - k0 - 32 * c);
-        const uint64_t dl2 = f32x2(stat.y, stat.y), sc2 = f32x2(p.scale_log2, p.scale_log2), nl2 = f32x2(-stat.x, -stat.x);
+        const uint64_t dl2 = f32x2(stat.y, stat.y), sc2 = f32x2(p.scale_log2, p.scale_log2), nl2 = f32x2(-from, -from);
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float2 y = f32x2_split(fma_f32x2(f32x2(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), sc2, nl2));
@@ -1184,12 +1265,16 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
     {
       float* sums = reinterpret_cast<float*>(smem + C::oSum);
       const float2 e2 = f32x2_split(exact);
-      const float mine = e2.x + e2.y;
+      const float mine = (e2.x + e2.y) * power_of_2(-up);
       if (half == 1) sums[256 + r] = mine;
       mbar_arrive(sums_full);
       if (half == 0) {
         ok = mbar_wait_warp(sums_full, 0, kBudgetNs, abort_flag, status) && ok;
-        p.stat[(int64_t)h * p.Np + i] = make_float2(-stat.x, real ? -(mine + sums[256 + r]) : 0.f);
+        const float delta = real ? mine + sums[256 + r] : 0.f;
+        p.stat[(int64_t)h * p.Np + i] = make_float2(kUp<T> - stat.x, -delta);
+        if constexpr (kScaled<T>)
+          p.d_most[(int64_t)h * p.Np + i] = make_float2(most_of_seq(norm, seq),
+                                                        most_of_seq(fabsf(delta) < INFINITY ? fabsf(delta) : 0.f, seq));
       }
     }
     if (ok && mbar_wait_warp(done, 0, kBudgetNs, abort_flag, status)) {
@@ -1197,7 +1282,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       bool odd = false;
 #pragma unroll 1
       for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c)  // through the ring's memory, which is free by now
-        odd |= store_cols<T>(lane_base + 256 + c * 32, p.scale, p.dq, &maps.dq, maps.swap_dq,
+        odd |= store_cols<T>(lane_base + 256 + c * 32, p.scale * power_of_2(-up), p.dq, &maps.dq, maps.swap_dq,
                              smem + C::oK + (warp - 4) * kOutBytes, c * 32, h, i, lane, real, p.N);
       // as in the forward: no number, though the scores are, and foreign keys among the tile's that were not cleared
       bool again = real && odd && stat.x == stat.x;
@@ -1376,11 +1461,40 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
     // the queries that see this key row (none for a row of no sequence)
     const bool real = j < p.N && __ldg(p.start + j) <= j && queries_of(p, j) > j;
     const int q_hi = real ? queries_of(p, j) : 0;
-    const int z = __ldg(p.end + k_last);  // queries from here on are foreign to every key of the tile: all in block qb_hi
     bool ok = true;
+    int up = 0;  // dS goes to its product times 2^up
+    if constexpr (kScaled<T>) {
+      ok = mbar_wait_warp(kv_full, 0, kBudgetNs, abort_flag, status);
+      if (!ok) fail(kErrTimeoutEpilogue);
+      float v2 = 0.f;  // |v_j|^2
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 a = *reinterpret_cast<const uint4*>(smem + C::oV + (c >> 3) * kAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = Half16<T>::unpack(w[e]);
+          v2 = fmaf(f.x, f.x, fmaf(f.y, f.y, v2));
+        }
+      }
+      // the 32 rows with this one among them; behind them, rows of one sequence alone see these: that of their last row
+      const int g0 = j - lane, hi = __reduce_max_sync(0xffffffffu, q_hi);
+      float2 own = make_float2(0.f, 0.f), behind = own;
+      auto take = [](float2& m, float2 x) { m = make_float2(fmaxf(m.x, x.x), fmaxf(m.y, x.y)); };
+      for (int h = kvh * group; h < (kvh + 1) * group; ++h) {
+        const float2* most = p.d_most + (int64_t)h * p.Np;
+        for (int i = g0 + 32 + lane * 32; i < hi; i += 32 * 32) take(behind, most[i]);
+        if (real) take(own, most[j]);
+      }
+      behind = make_float2(warp_max(behind.x), warp_max(behind.y));
+      if (q_hi > g0 + 32) take(own, behind);
+      up = up_for(own.x * (v2 < INFINITY ? sqrtf(v2) : 0.f) + own.y);
+    }
+    const float more = power_of_2(up - (int)kUp<T>);  // P has kUp already
+    const int z = __ldg(p.end + k_last);  // queries from here on are foreign to every key of the tile: all in block qb_hi
     const uint32_t set_base = lane_base + half * 128;
     int qb = half % nq;  // the iteration's query block, counted from qb_lo
-    for (int it = half; it < iters; it += 2) {
+    for (int it = half; ok && it < iters; it += 2) {
       const int st = it % C::kStages;
       if (!mbar_wait_warp(&s_full[half], (it >> 1) & 1, kBudgetNs, abort_flag, status)) {
         fail(kErrTimeoutEpilogue);
@@ -1419,6 +1533,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
             g.x = v0 ? g.x : 0.f;
             g.y = v1 ? g.y : 0.f;
           }
+          if constexpr (kScaled<T>) g = f32x2_split(mul_f32x2(f32x2(g.x, g.y), f32x2(more, more)));
           pp[c * 16 + e / 2] = Half16<T>::pack(p0, p1);
           ss[c * 16 + e / 2] = Half16<T>::pack(g.x, g.y);
         }
@@ -1454,7 +1569,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       bool odd = false;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c)
-        odd |= store_cols<T>(lane_base + (half ? 384 : 256) + c * 32, half ? p.scale : 1.f, to, half ? &maps.dk : &maps.dv,
+        odd |= store_cols<T>(lane_base + (half ? 384 : 256) + c * 32, half ? p.scale * power_of_2(-up) : power_of_2(-(int)kUp<T>), to, half ? &maps.dk : &maps.dv,
                              (maps.swap_o >> half) & 1, smem + C::oQ + (warp - 4) * kOutBytes, c * 32, kvh, j, lane, real,
                              p.N);
       // no number, and foreign queries among the tile's that were not cleared
@@ -1649,15 +1764,17 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
   torch::Tensor dq = out_rows(dq_, what, "dq", H, q), dk = out_rows(dk_, what, "dk", KV, q),
                 dv = out_rows(dv_, what, "dv", KV, q);
   p.Np = (int)((N + BT - 1) / BT * BT);
+  const bool scaled = q.scalar_type() == at::kHalf;
+  const int64_t entries = (int64_t)p.Np * (scaled ? 4 * H + KV : 2 * H);
   torch::Tensor scratch;
   if (scratch_.has_value() && scratch_->defined()) {
     scratch = *scratch_;
-    TORCH_CHECK_VALUE(scratch.scalar_type() == at::kFloat && scratch.is_contiguous() && scratch.numel() >= 2 * H * p.Np &&
+    TORCH_CHECK_VALUE(scratch.scalar_type() == at::kFloat && scratch.is_contiguous() && scratch.numel() >= entries &&
                           reinterpret_cast<uintptr_t>(scratch.data_ptr()) % 16 == 0,
-                      what, ": scratch must be contiguous float32 of ", std::to_string(2 * H * p.Np), " entries, 16-byte aligned");
+                      what, ": scratch must be contiguous float32 of ", std::to_string(entries), " entries, 16-byte aligned");
     TORCH_CHECK_VALUE(scratch.device() == q.device(), what, ": scratch is on another device than q");
   } else {
-    scratch = torch::empty({2 * H * p.Np}, q.options().dtype(at::kFloat));
+    scratch = torch::empty({entries}, q.options().dtype(at::kFloat));
   }
   at::assert_no_overlap(dq, dk);
   at::assert_no_overlap(dq, dv);
@@ -1673,6 +1790,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
   p.dv = rows_of(dv);
   p.lse = lse.data_ptr<float>();
   p.stat = reinterpret_cast<float2*>(scratch.data_ptr<float>());
+  p.d_most = p.stat + H * p.Np;
+  p.v_most = reinterpret_cast<float*>(p.d_most + H * p.Np);
   c10::cuda::CUDAGuard g(q.device());
   auto st = at::cuda::getCurrentCUDAStream();
   by_type(q, [&](auto t, auto d) {
@@ -1697,6 +1816,10 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
     const int64_t tiles = p.Np / BT;
     TORCH_CHECK_VALUE(tiles * H < (int64_t(1) << 31), what, ": too many rows or heads");
     int* status = status_ptr(q.device().index());
+    if constexpr (kScaled<T>) {
+      v_most_kernel<T, D><<<(unsigned)((p.Np / 32 * KV + kNormThreads / 32 - 1) / (kNormThreads / 32)), kNormThreads, 0, st>>>(p);
+      C10_CUDA_KERNEL_LAUNCH_CHECK();
+    }
     dq_tc_kernel<T, D><<<(unsigned)(tiles * H), kThreads, DqCfg<D>::kSmem, st>>>(a, p, status);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     dkv_tc_kernel<T, D><<<(unsigned)(tiles * KV), kThreads, DkvCfg<D>::kSmem, st>>>(b, p, status);
