@@ -6,8 +6,9 @@ sequence (padding) has the empty span ``[i, i)``. The spans come from the sequen
 which each document starts with BOS, are made once per batch, and serve the forward and backward of every layer.
 
 Row ``i`` sees the rows ``j`` of its sequence with ``i - window < j <= i`` (``window=0``: all up to ``i``).
-Nothing of one sequence reaches another one's results, values that are no numbers included, nor does what the
-padding rows hold; rows of no sequence are left as they were in every output (zero in one that the call makes).
+What a row does not see (other sequences, later rows, rows outside its window, padding rows) does not reach its results,
+values that are no numbers included, nor do queries that do not see a key reach that key's gradients; rows of no
+sequence are left as they were in every output (zero in one that the call makes).
 Spans must be those of sequences that follow one another; any other contents give wrong values but read and
 write no row outside the tensors.
 

@@ -16,20 +16,23 @@
 // short sequences fills them as well as one long sequence does, no work list has to be built, and the sequences
 // appear only as each row's range of keys. A matrix product multiplies hidden keys by a weight of exactly 0,
 // which does nothing unless such a key holds a value that is no number. Keys before the first sequence of a
-// work item are overwritten with zeros in shared memory; what else is foreign to a row is within its own
-// tiles' rows: a row that came out as no number and has such keys is computed alone, from its own keys
-// (fwd_row). That can be the case only within 256 rows of a border, so its cost stays bounded.
+// work item are overwritten with zeros in shared memory; what else a row does not see is within the item's own
+// tiles' rows: a row that came out as no number, and has foreign keys or hidden ones of its own sequence that are
+// no numbers there, has those columns computed alone, from its own keys (fwd_row). A row's hidden keys of its own
+// sequence are less than 256 rows away, and where the keys that it sees make it no number the computation ends with
+// the first that does in all those columns, so the cost stays bounded also where all values are none.
 //
 // Backward: dQ, then dK/dV, on tcgen05 tiles of the same kind (described at the kernels).
 //
 // Row by row (the rows that a tile's product spoils): one warp per row and head, a lane holds D / 32 of the row's
-// values in fp32, a score is a warp-wide sum.
+// values in fp32, a score is a warp-wide sum. Only columns that came out as no numbers are written again.
 #include <torch/extension.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <atomic>
+#include <climits>
 #include <string>
 #include <tuple>
 #include <utility>
@@ -104,6 +107,57 @@ __device__ __forceinline__ void store_row(const Rows& r, int64_t i, int h, int l
     *reinterpret_cast<uint32_t*>(p) = Half16<T>::pack(x[0], x[1]);
   }
 }
+__device__ __forceinline__ bool is_number(float x) { return fabsf(x) < INFINITY; }
+// the columns of a row that the tiles' product left as no numbers, and the row as it stands. Its values were written by
+// other lanes before a __syncwarp (by bulk copies: before lane 0 had waited for them)
+template <typename T, int D>
+__device__ __forceinline__ uint32_t spoilt_columns(const Rows& r, int64_t i, int h, int lane, float (&x)[D / 32]) {
+  const T* p = reinterpret_cast<const T*>(r.p) + i * r.row + h * r.head + lane * (D / 32);
+  uint32_t u[D / 64], need = 0;
+  if constexpr (D == 128) {
+    const uint2 w = __ldcg(reinterpret_cast<const uint2*>(p));
+    u[0] = w.x, u[1] = w.y;
+  } else {
+    u[0] = __ldcg(reinterpret_cast<const uint32_t*>(p));
+  }
+#pragma unroll
+  for (int e = 0; e < D / 32; e += 2) {
+    const float2 f = Half16<T>::unpack(u[e / 2]);
+    x[e] = f.x, x[e + 1] = f.y;
+    need |= (uint32_t)!is_number(f.x) << e | (uint32_t)!is_number(f.y) << (e + 1);
+  }
+  return need;
+}
+// every column that is needed is NaN: nothing that is added to them changes that
+template <int E>
+__device__ __forceinline__ bool all_lost(const float (&acc)[E], uint32_t need) {
+  bool lost = true;
+#pragma unroll
+  for (int e = 0; e < E; ++e) lost &= !((need >> e) & 1u) || acc[e] != acc[e];
+  return __all_sync(0xffffffffu, lost);
+}
+// The first and the last of the rows [lo, hi) that hold a value that is no number in one of the heads [h0, h1)
+// ((INT_MAX, -1): none). The whole warp.
+template <typename T, int D>
+__device__ __noinline__ int2 odd_rows(const Rows& r, int h0, int h1, int lo, int hi, int lane) {
+  constexpr uint32_t kExp = Half16<T>::kFormat ? 0x7f80u : 0x7c00u;
+  int first = INT_MAX, last = -1;
+  for (int i = lo + lane; i < hi; i += 32) {
+    bool odd = false;
+    for (int h = h0; h < h1; ++h) {
+      const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(r.p) + (int64_t)i * r.row + h * r.head);
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 a = __ldg(p + c);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= (w[e] & kExp) == kExp || ((w[e] >> 16) & kExp) == kExp;
+      }
+    }
+    if (odd) first = min(first, i), last = i;
+  }
+  return make_int2(__reduce_min_sync(0xffffffffu, first), __reduce_max_sync(0xffffffffu, last));
+}
 template <int E>
 __device__ __forceinline__ float dot(const float (&a)[E], const float (&b)[E]) {
   float s = 0.f;
@@ -130,22 +184,24 @@ __device__ __noinline__ void fwd_row(const PackedParams& p, int i, int h, int la
   const int2 key = keys_of(p, i);
   if (key.y <= key.x) return;
   const int g = h / (p.H / p.KV);
-  float q[E], acc[E] = {};
+  float q[E], old[E], acc[E] = {};
+  const uint32_t need = spoilt_columns<T, D>(p.o, i, h, lane, old);
   load_row<T, D>(p.q, i, h, lane, q);
   float m = -INFINITY, l = 0.f;
-  for (int j0 = key.x; j0 < key.y; j0 += 4) {  // four keys at a time: their loads overlap
+  // from the last key on: behind one that is no number there usually are more
+  for (int j0 = key.y - 1; j0 >= key.x && !all_lost(acc, need); j0 -= 4) {  // four keys at a time: their loads overlap
     float v[4][E], x[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       float k[E];
-      const int j = min(j0 + u, key.y - 1);
+      const int j = max(j0 - u, key.x);
       load_row<T, D>(p.k, j, g, lane, k);
       load_row<T, D>(p.v, j, g, lane, v[u]);
       x[u] = dot(q, k) * p.scale_log2;
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (j0 + u >= key.y) break;
+      if (j0 - u < key.x) break;
       if (x[u] > m) {  // the same in every lane
         const float a = exp2f(m - x[u]);
         l *= a;
@@ -161,9 +217,8 @@ __device__ __noinline__ void fwd_row(const PackedParams& p, int i, int h, int la
   }
   const float inv = 1.f / l;
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] *= inv;
-  store_row<T, D>(p.o, i, h, lane, acc);
-  if (lane == 0) p.lse[(int64_t)h * p.N + i] = (m + log2f(l)) * kLn2;
+  for (int e = 0; e < E; ++e) acc[e] = (need >> e) & 1u ? acc[e] * inv : old[e];
+  store_row<T, D>(p.o, i, h, lane, acc);  // its lse is right: hidden scores are not added up
 }
 
 template <typename T, int D>
@@ -172,37 +227,42 @@ __device__ __noinline__ void dq_row(const PackedParams& p, int i, int h, int hal
   const int2 key = keys_of(p, i);
   if (key.y <= key.x) return;
   const int g = h / (p.H / p.KV);
-  float q[E], d[E], acc[E] = {};
+  float q[E], d[E], old[E], acc[E] = {};
+  // the other half of the row is the other warp's
+  const uint32_t need = lane / 16 == half ? spoilt_columns<T, D>(p.dq, i, h, lane, old) : 0u;
   load_row<T, D>(p.q, i, h, lane, q);
   load_row<T, D>(p.dout, i, h, lane, d);
-  for (int j0 = key.x; j0 < key.y; j0 += 4) {  // four keys at a time: their loads overlap
+  for (int j0 = key.y - 1; j0 >= key.x && !all_lost(acc, need); j0 -= 4) {  // four keys at a time: their loads overlap
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       float k[E], v[E];
-      const int j = min(j0 + u, key.y - 1);
+      const int j = max(j0 - u, key.x);
       load_row<T, D>(p.k, j, g, lane, k);
       load_row<T, D>(p.v, j, g, lane, v);
       const float w = exp2f(dot(q, k) * p.scale_log2 - stat.x);
       const float ds = w * (dot(d, v) - stat.y);
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = j0 + u < key.y ? fmaf(ds, k[e], acc[e]) : acc[e];
+      for (int e = 0; e < E; ++e) acc[e] = j0 - u >= key.x ? fmaf(ds, k[e], acc[e]) : acc[e];
     }
   }
+  if (lane / 16 != half) return;
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] *= p.scale;
-  if (lane / 16 == half) store_row<T, D>(p.dq, i, h, lane, acc);  // the other half of the row is the other warp's
+  for (int e = 0; e < E; ++e) acc[e] = (need >> e) & 1u ? acc[e] * p.scale : old[e];
+  store_row<T, D>(p.dq, i, h, lane, acc);
 }
 
 template <typename T, int D>
 __device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool want_dk, int lane) {
   constexpr int E = D / 32;
   const int hi = queries_of(p, j), group = p.H / p.KV;
-  float k[E], v[E], acc[E] = {};
+  const Rows& to = want_dk ? p.dk : p.dv;
+  float k[E], v[E], old[E], acc[E] = {};
+  const uint32_t need = spoilt_columns<T, D>(to, j, g, lane, old);
   load_row<T, D>(p.k, j, g, lane, k);
   load_row<T, D>(p.v, j, g, lane, v);
-  for (int h = g * group; h < (g + 1) * group; ++h) {
-    const float2* stat = p.stat + (int64_t)h * p.Np;
-    for (int i0 = j; i0 < hi; i0 += 4) {
+  for (int i0 = j; i0 < hi && !all_lost(acc, need); i0 += 4) {
+    for (int h = g * group; h < (g + 1) * group; ++h) {
+      const float2* stat = p.stat + (int64_t)h * p.Np;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         float q[E], d[E];
@@ -217,15 +277,10 @@ __device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool w
       }
     }
   }
-  if (want_dk) {
+  const float f = (want_dk ? p.scale : 1.f) * power_of_2(-(int)kUp<T>);  // stat raised the weights
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] *= p.scale;
-  }
-  if constexpr (kScaled<T>) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] *= power_of_2(-(int)kUp<T>);  // stat raised the weights
-  }
-  store_row<T, D>(want_dk ? p.dk : p.dv, j, g, lane, acc);
+  for (int e = 0; e < E; ++e) acc[e] = (need >> e) & 1u ? acc[e] * f : old[e];
+  store_row<T, D>(to, j, g, lane, acc);
 }
 
 // the largest of the values (none negative) of a warp's lanes that have the same seq
@@ -867,11 +922,17 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
         __syncwarp();
       }
       if (real) p.lse[(int64_t)h * p.N + i] = (m_ref + log2f(l)) * kLn2;
-      // rows that are no numbers although their scores are, and whose tiles hold foreign keys that were not cleared
+      // rows that are no numbers although their scores are, and whose tiles hold foreign keys that were not cleared, or
+      // hidden keys of the row's own sequence that are no numbers
       bool again = real && odd != 0.f && l == l;
-      if (again) {
+      if (__any_sync(0xffffffffu, again)) {
         const int first = t_lo == t0 ? max(t_lo * BB, z) : t_lo * BB;
-        again = __ldg(p.start + i) > first || __ldg(p.end + i) < t_hi * BB;
+        const bool foreign = again && (__ldg(p.start + i) > first || __ldg(p.end + i) < t_hi * BB);
+        const bool own = again && !foreign;
+        const int g = h / (p.H / p.KV), row0 = i - lane;
+        const int later = odd_rows<T, D>(p.v, g, g + 1, row0 + 1, min(t_hi * BB, p.N), lane).y;
+        const int earlier = odd_rows<T, D>(p.v, g, g + 1, first, __reduce_max_sync(0xffffffffu, own ? key.x : 0), lane).x;
+        again = foreign || (own && (later >= key.y || earlier < key.x));
       }
       uint32_t redo = __ballot_sync(0xffffffffu, again);
       if (redo) {
@@ -1284,9 +1345,17 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
       for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c)  // through the ring's memory, which is free by now
         odd |= store_cols<T>(lane_base + 256 + c * 32, p.scale * power_of_2(-up), p.dq, &maps.dq, maps.swap_dq,
                              smem + C::oK + (warp - 4) * kOutBytes, c * 32, h, i, lane, real, p.N);
-      // as in the forward: no number, though the scores are, and foreign keys among the tile's that were not cleared
-      bool again = real && odd && stat.x == stat.x;
-      if (again) again = __ldg(p.start + i) > max(kb_lo * BB, z) || __ldg(p.end + i) < (kb_hi + 1) * BB;
+      // as in the forward: no number, though the scores and delta are, and foreign keys among the tile's that were not
+      // cleared, or hidden ones that are no numbers
+      bool again = real && odd && stat.x == stat.x && is_number(stat.y);
+      if (__any_sync(0xffffffffu, again)) {
+        const int first = max(kb_lo * BB, z);
+        const bool foreign = again && (__ldg(p.start + i) > first || __ldg(p.end + i) < (kb_hi + 1) * BB);
+        const bool own = again && !foreign;
+        const int later = odd_rows<T, D>(p.k, kvh, kvh + 1, i - lane + 1, min((kb_hi + 1) * BB, p.N), lane).y;
+        const int earlier = odd_rows<T, D>(p.k, kvh, kvh + 1, first, __reduce_max_sync(0xffffffffu, own ? key.x : 0), lane).x;
+        again = foreign || (own && (later >= key.y || earlier < key.x));
+      }
       uint32_t redo = __ballot_sync(0xffffffffu, again);
       if (lane == 0) out_wait_done();  // also before any row's second values
       __syncwarp();
@@ -1572,9 +1641,18 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
         odd |= store_cols<T>(lane_base + (half ? 384 : 256) + c * 32, half ? p.scale * power_of_2(-up) : power_of_2(-(int)kUp<T>), to, half ? &maps.dk : &maps.dv,
                              (maps.swap_o >> half) & 1, smem + C::oQ + (warp - 4) * kOutBytes, c * 32, kvh, j, lane, real,
                              p.N);
-      // no number, and foreign queries among the tile's that were not cleared
+      // no number, and foreign queries among the tile's that were not cleared, or hidden ones that are no numbers
       bool again = real && odd;
-      if (again) again = __ldg(p.start + j) > k0 || __ldg(p.end + j) < min(z, (qb_hi + 1) * BB);
+      if (__any_sync(0xffffffffu, again)) {
+        const int end = min(z, (qb_hi + 1) * BB);
+        const bool foreign = again && (__ldg(p.start + j) > k0 || __ldg(p.end + j) < end);
+        const bool own = again && !foreign;
+        const Rows& from = half ? p.q : p.dout;  // what the hidden weights of 0 are multiplied by
+        const int earlier = odd_rows<T, D>(from, kvh * group, (kvh + 1) * group, k0, min(j - lane + 31, p.N), lane).x;
+        const int later = odd_rows<T, D>(from, kvh * group, (kvh + 1) * group,
+                                         __reduce_min_sync(0xffffffffu, own ? q_hi : p.N), min(end, p.N), lane).y;
+        again = foreign || (own && (earlier < j || later >= q_hi));
+      }
       uint32_t redo = __ballot_sync(0xffffffffu, again);
       if (lane == 0) out_wait_done();  // also before any row's second values
       __syncwarp();
