@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = warp_id();
-  if (device_failed(status)) return;
+  if (__syncthreads_or(device_failed(status))) return;  // all threads or none: the word may change meanwhile
   if (threadIdx.x == 0) {
     for (int x = 0; x < 2; ++x) {
       mbar_init(&q_full[x], 1);
@@ -1063,7 +1063,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
   const int tile = (int)gridDim.x / p.H - 1 - (int)blockIdx.x / p.H, h = blockIdx.x % p.H;  // late rows first
   const int kvh = h / (p.H / p.KV), q0 = tile * BT;
   const int warp = warp_id();
-  if (device_failed(status)) return;
+  if (__syncthreads_or(device_failed(status))) return;  // all threads or none: the word may change meanwhile
   // spans never decrease along the rows: the first row has the first key
   const int kb_hi = min(q0 + BT, p.N) - 1 >> 6;
   const int kb_lo = min(max(keys_of(p, q0).x, 0) >> 6, kb_hi);
@@ -1416,7 +1416,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
 
   const int kvh = blockIdx.x % p.KV, k0 = (int)blockIdx.x / p.KV * BT, group = p.H / p.KV;
   const int warp = warp_id();
-  if (device_failed(status)) return;
+  if (__syncthreads_or(device_failed(status))) return;  // all threads or none: the word may change meanwhile
   // spans never decrease along the rows: the last row is seen by the last query
   const int k_last = min(k0 + BT, p.N) - 1;
   const int qb_lo = k0 / BB, qb_hi = (max(queries_of(p, k_last), k_last + 1) - 1) / BB;
