@@ -37,7 +37,7 @@ def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     ``grad`` may be given, also as ``logits`` itself (in place). ``need_grad=False`` returns the loss alone. Runs on
     the current stream of the logits' device, in a captured graph too (once any kernel of this package has run on
     that device); the same inputs give the same bits. Wrong arguments raise
-    ``ValueError``."""
+    ``ValueError``, a ``grad`` that shares memory with another argument otherwise ``RuntimeError``."""
     if scale is None:
         scale = 1.0 / max(1, logits.shape[0])
     return ext().distill_topk(logits, teacher_ids, teacher_logits, targets, cap, temperature, alpha, scale, need_grad,

@@ -14,7 +14,8 @@ write no row outside the tensors.
 
 Calls run on the current stream of the tensors' device, in a captured graph too (once any kernel of this package
 has run on that device), allocate only the outputs and the
-backward's scratch when they are not given, and give the same bits for the same inputs. Wrong arguments raise ``ValueError``.
+backward's scratch when they are not given, and give the same bits for the same inputs. Wrong arguments raise ``ValueError``, outputs that
+share memory with another argument ``RuntimeError``.
 As with the other tensor-core kernels, results count only while the device status word is zero (``check_status``): once it
 holds an error, attention calls leave their outputs as they were.
 """

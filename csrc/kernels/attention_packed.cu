@@ -27,7 +27,6 @@
 // Row by row (the rows that a tile's product spoils): one warp per row and head, a lane holds D / 32 of the row's
 // values in fp32, a score is a warp-wide sum. Only columns that came out as no numbers are written again.
 #include <torch/extension.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -38,6 +37,7 @@
 #include <utility>
 
 #include "half_types.cuh"
+#include "overlap.h"
 #include "status.h"
 #include "tma_host.h"
 
@@ -1699,7 +1699,6 @@ torch::Tensor out_rows(const c10::optional<torch::Tensor>& t, const char* what, 
   // rows of no sequence are left as they were: in a new tensor they are zero
   if (!t.has_value() || !t->defined()) return torch::zeros({like.size(0), heads, like.size(2)}, like.options());
   check_rows(*t, what, name, like.size(0), heads, like.size(2), like);
-  at::assert_no_internal_overlap(*t);
   return *t;
 }
 
@@ -1800,7 +1799,8 @@ std::tuple<torch::Tensor, torch::Tensor> packed_attn_fwd(const torch::Tensor& q,
   PackedParams p = common_params(what, q, k, v, start, end, window, scale);
   torch::Tensor out = out_rows(out_, what, "out", p.H, q);
   torch::Tensor lse = stat_rows(lse_, what, "lse", p.H, q, true);
-  for (const torch::Tensor* t : {&q, &k, &v}) at::assert_no_overlap(out, *t);
+  check_output(what, {"out", &out}, {{"q", &q}, {"k", &k}, {"v", &v}, {"start", &start}, {"end", &end}});
+  check_output(what, {"lse", &lse}, {{"out", &out}, {"q", &q}, {"k", &k}, {"v", &v}, {"start", &start}, {"end", &end}});
   TORCH_CHECK_VALUE(q.is_cuda(), what, ": q must be on a CUDA device");
   if (p.N == 0) return {out, lse};
   p.o = rows_of(out);
@@ -1854,11 +1854,12 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> packed_attn_bwd(
   } else {
     scratch = torch::empty({entries}, q.options().dtype(at::kFloat));
   }
-  at::assert_no_overlap(dq, dk);
-  at::assert_no_overlap(dq, dv);
-  at::assert_no_overlap(dk, dv);
-  for (const torch::Tensor* r : {&dq, &dk, &dv})
-    for (const torch::Tensor* t : {&q, &k, &v, &out, &dout}) at::assert_no_overlap(*r, *t);
+  for (const Named& r : {Named("dq", &dq), Named("dk", &dk), Named("dv", &dv), Named("scratch", &scratch)})
+    check_output(what, r, {{"q", &q}, {"k", &k}, {"v", &v}, {"out", &out}, {"lse", &lse}, {"dout", &dout},
+                           {"start", &start}, {"end", &end}});
+  check_output(what, {"dq", &dq}, {{"dk", &dk}, {"dv", &dv}, {"scratch", &scratch}});
+  check_output(what, {"dk", &dk}, {{"dv", &dv}, {"scratch", &scratch}});
+  check_output(what, {"dv", &dv}, {{"scratch", &scratch}});
   TORCH_CHECK_VALUE(q.is_cuda(), what, ": q must be on a CUDA device");
   if (N == 0) return {dq, dk, dv};
   p.o = rows_of(out);

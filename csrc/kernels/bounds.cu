@@ -11,6 +11,7 @@
 #include <tuple>
 
 #include "common.cuh"
+#include "overlap.h"
 #include "status.h"
 
 namespace br {
@@ -151,6 +152,8 @@ std::tuple<torch::Tensor, torch::Tensor> bounds_from_offsets(const torch::Tensor
                     "bounds_from_offsets: offsets needs at least one entry");
   TORCH_CHECK_VALUE(rows >= 0 && rows < (int64_t(1) << 31), "bounds_from_offsets: rows out of range");
   torch::Tensor start = bounds_out(start_out, rows, offsets, "start"), end = bounds_out(end_out, rows, offsets, "end");
+  check_output("bounds_from_offsets", {"start", &start}, {{"end", &end}, {"offsets", &offsets}});
+  check_output("bounds_from_offsets", {"end", &end}, {{"offsets", &offsets}});
   TORCH_CHECK_VALUE(offsets.is_cuda(), "bounds_from_offsets: offsets must be on a CUDA device");
   c10::cuda::CUDAGuard g(offsets.device());
   if (rows == 0) return {start, end};
@@ -171,6 +174,8 @@ std::tuple<torch::Tensor, torch::Tensor> bounds_from_ids(const torch::Tensor& id
   TORCH_CHECK_VALUE(rows < (int64_t(1) << 31), "bounds_from_ids: too many tokens");
   TORCH_CHECK_VALUE(bos >= INT32_MIN && bos <= INT32_MAX, "bounds_from_ids: bos is not an int32");
   torch::Tensor start = bounds_out(start_out, rows, ids, "start"), end = bounds_out(end_out, rows, ids, "end");
+  check_output("bounds_from_ids", {"start", &start}, {{"end", &end}, {"ids", &ids}});
+  check_output("bounds_from_ids", {"end", &end}, {{"ids", &ids}});
   TORCH_CHECK_VALUE(ids.is_cuda(), "bounds_from_ids: ids must be on a CUDA device");
   c10::cuda::CUDAGuard g(ids.device());
   if (rows == 0) return {start, end};

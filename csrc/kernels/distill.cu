@@ -29,7 +29,6 @@
 // 306 us (3.5 TB/s; 22 instructions per logit, a row's fixed part among them, fill half of the issue slots). With
 // one block per row, no ring and no entries' warps it was 378 us there, and 690 us for the wide rows.
 #include <torch/extension.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -38,6 +37,7 @@
 #include <tuple>
 
 #include "half_types.cuh"
+#include "overlap.h"
 #include "status.h"
 
 namespace br {
@@ -690,10 +690,12 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> distill_t
                             grad_->scalar_type() == logits.scalar_type() && grad_->device() == logits.device() &&
                             (V == 1 || grad_->stride(1) == 1) && (M <= 1 || grad_->stride(0) >= V), what,
                         "grad must be [M, V] like the logits, with contiguous rows");
-      // the logits themselves (in place), or apart from them
-      if (!(grad_->data_ptr() == logits.data_ptr() && grad_->strides() == logits.strides()))
-        at::assert_no_overlap(*grad_, logits);
       grad = *grad_;
+      // the logits themselves (in place), or apart from them
+      if (grad->data_ptr() != logits.data_ptr() || (M > 1 && grad->stride(0) != logits.stride(0)))
+        check_output("distill_topk", {"grad", &*grad}, {{"logits", &logits}});
+      check_output("distill_topk", {"grad", &*grad}, {{"teacher_ids", &ids}, {"teacher_logits", &teacher}});
+      if (has_targets) check_output("distill_topk", {"grad", &*grad}, {{"targets", &*targets}});
     } else {
       grad = torch::empty({M, V}, logits.options());
     }
