@@ -24,8 +24,9 @@
 //
 // Backward: dQ, then dK/dV, on tcgen05 tiles of the same kind (described at the kernels).
 //
-// Row by row (the rows that a tile's product spoils): one warp per row and head, a lane holds D / 32 of the row's
-// values in fp32, a score is a warp-wide sum. Only columns that came out as no numbers are written again.
+// Row by row (the rows that a tile's product spoils): one warp per row and head, 32 keys (or queries) at a time: each
+// lane takes the dot products of one of them with the row's vectors, which lie in shared memory, then each lane adds up
+// D / 32 columns of all 32. Only columns that came out as no numbers are written again.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -64,6 +65,7 @@ struct PackedParams {
   float* v_most;   // [KV, Np]: |v|
   float2* d_most;  // [H, Np]: |do| and |delta|
   int Np;        // N rounded up to whole tiles
+  uint64_t wait_ns;  // how long a wait of the forward may take: rows by themselves hold a tile up
 };
 
 // Powers of two that keep the fp16 backward's 16-bit factors in the normal range. P of a long sequence is far below
@@ -166,6 +168,43 @@ __device__ __forceinline__ float dot(const float (&a)[E], const float (&b)[E]) {
   return warp_sum(s);
 }
 
+// x[0..D) in shared memory, as fp32 times f, from the lanes' parts of a row
+template <int E>
+__device__ __forceinline__ void keep_row(float* x, int lane, const float (&v)[E], float f) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[lane * E + e] = v[e] * f;
+}
+// one lane's dot product of row (i, h) with x
+template <typename T, int D>
+__device__ __forceinline__ float dot_row(const Rows& r, int64_t i, int h, const float* x) {
+  const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(r.p) + i * r.row + h * r.head);
+  float s[2] = {};
+#pragma unroll 8
+  for (int c = 0; c < D / 8; ++c) {
+    const uint4 a = __ldg(p + c);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = Half16<T>::unpack(w[e]), y = *reinterpret_cast<const float2*>(x + c * 8 + 2 * e);
+      s[e & 1] = fmaf(f.x, y.x, fmaf(f.y, y.y, s[e & 1]));
+    }
+  }
+  return s[0] + s[1];
+}
+// acc += sum of w_u times row (first + u step) of r, w_u lane u's, over the rows u < count
+template <typename T, int D>
+__device__ __forceinline__ void add_rows(const Rows& r, int first, int step, int count, int h, float w, int lane,
+                                         float (&acc)[D / 32]) {
+#pragma unroll 8
+  for (int u = 0; u < count; ++u) {
+    float v[D / 32];
+    load_row<T, D>(r, first + u * step, h, lane, v);
+    const float wu = __shfl_sync(0xffffffffu, w, u);
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(wu, v[e], acc[e]);
+  }
+}
+
 // the keys that row i sees, [lo, hi)
 __device__ __forceinline__ int2 keys_of(const PackedParams& p, int i) {
   const int lo = max(max(__ldg(p.start + i), 0), i - p.window + 1);
@@ -179,7 +218,7 @@ __device__ __forceinline__ int queries_of(const PackedParams& p, int j) {
 }
 
 template <typename T, int D>
-__device__ __noinline__ void fwd_row(const PackedParams& p, int i, int h, int lane) {
+__device__ __noinline__ void fwd_row(const PackedParams& p, int i, int h, int lane, float* buf) {
   constexpr int E = D / 32;
   const int2 key = keys_of(p, i);
   if (key.y <= key.x) return;
@@ -187,64 +226,52 @@ __device__ __noinline__ void fwd_row(const PackedParams& p, int i, int h, int la
   float q[E], old[E], acc[E] = {};
   const uint32_t need = spoilt_columns<T, D>(p.o, i, h, lane, old);
   load_row<T, D>(p.q, i, h, lane, q);
-  float m = -INFINITY, l = 0.f;
+  keep_row(buf, lane, q, p.scale_log2);
+  __syncwarp();
+  float m = -INFINITY, l = 0.f;  // l: this lane's keys
   // from the last key on: behind one that is no number there usually are more
-  for (int j0 = key.y - 1; j0 >= key.x && !all_lost(acc, need); j0 -= 4) {  // four keys at a time: their loads overlap
-    float v[4][E], x[4];
+  for (int last = key.y - 1; last >= key.x && !all_lost(acc, need); last -= 32) {
+    const int j = last - lane, count = min(32, last - key.x + 1);
+    const float x = lane < count ? dot_row<T, D>(p.k, j, g, buf) : -INFINITY, most = warp_max(x);
+    if (most > m) {
+      const float a = exp2f(m - most);
+      l *= a;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float k[E];
-      const int j = max(j0 - u, key.x);
-      load_row<T, D>(p.k, j, g, lane, k);
-      load_row<T, D>(p.v, j, g, lane, v[u]);
-      x[u] = dot(q, k) * p.scale_log2;
+      for (int e = 0; e < E; ++e) acc[e] *= a;
+      m = most;
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (j0 - u < key.x) break;
-      if (x[u] > m) {  // the same in every lane
-        const float a = exp2f(m - x[u]);
-        l *= a;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] *= a;
-        m = x[u];
-      }
-      const float w = exp2f(x[u] - (m == -INFINITY ? 0.f : m));  // a score of -inf has weight 0 also before any other
-      l += w;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[u][e], acc[e]);
-    }
+    const float w = exp2f(x - (m == -INFINITY ? 0.f : m));  // a score of -inf has weight 0 also before any other
+    l += w;
+    add_rows<T, D>(p.v, last, -1, count, g, w, lane, acc);
   }
-  const float inv = 1.f / l;
+  const float inv = 1.f / warp_sum(l);
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = (need >> e) & 1u ? acc[e] * inv : old[e];
   store_row<T, D>(p.o, i, h, lane, acc);  // its lse is right: hidden scores are not added up
+  __syncwarp();
 }
 
 template <typename T, int D>
-__device__ __noinline__ void dq_row(const PackedParams& p, int i, int h, int half, int lane, float2 stat) {
+__device__ __noinline__ void dq_row(const PackedParams& p, int i, int h, int half, int lane, float2 stat, float* buf) {
   constexpr int E = D / 32;
   const int2 key = keys_of(p, i);
   if (key.y <= key.x) return;
   const int g = h / (p.H / p.KV);
-  float q[E], d[E], old[E], acc[E] = {};
+  float x[E], old[E], acc[E] = {};
   // the other half of the row is the other warp's
   const uint32_t need = lane / 16 == half ? spoilt_columns<T, D>(p.dq, i, h, lane, old) : 0u;
-  load_row<T, D>(p.q, i, h, lane, q);
-  load_row<T, D>(p.dout, i, h, lane, d);
-  for (int j0 = key.y - 1; j0 >= key.x && !all_lost(acc, need); j0 -= 4) {  // four keys at a time: their loads overlap
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float k[E], v[E];
-      const int j = max(j0 - u, key.x);
-      load_row<T, D>(p.k, j, g, lane, k);
-      load_row<T, D>(p.v, j, g, lane, v);
-      const float w = exp2f(dot(q, k) * p.scale_log2 - stat.x);
-      const float ds = w * (dot(d, v) - stat.y);
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = j0 - u >= key.x ? fmaf(ds, k[e], acc[e]) : acc[e];
-    }
+  load_row<T, D>(p.q, i, h, lane, x);
+  keep_row(buf, lane, x, p.scale_log2);
+  load_row<T, D>(p.dout, i, h, lane, x);
+  keep_row(buf + D, lane, x, 1.f);
+  __syncwarp();
+  for (int last = key.y - 1; last >= key.x && !all_lost(acc, need); last -= 32) {
+    const int j = last - lane, count = min(32, last - key.x + 1);
+    float ds = 0.f;
+    if (lane < count) ds = exp2f(dot_row<T, D>(p.k, j, g, buf) - stat.x) * (dot_row<T, D>(p.v, j, g, buf + D) - stat.y);
+    add_rows<T, D>(p.k, last, -1, count, g, ds, lane, acc);
   }
+  __syncwarp();
   if (lane / 16 != half) return;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = (need >> e) & 1u ? acc[e] * p.scale : old[e];
@@ -252,35 +279,34 @@ __device__ __noinline__ void dq_row(const PackedParams& p, int i, int h, int hal
 }
 
 template <typename T, int D>
-__device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool want_dk, int lane) {
+__device__ __noinline__ void dkv_row(const PackedParams& p, int j, int g, bool want_dk, int lane, float* buf) {
   constexpr int E = D / 32;
   const int hi = queries_of(p, j), group = p.H / p.KV;
   const Rows& to = want_dk ? p.dk : p.dv;
-  float k[E], v[E], old[E], acc[E] = {};
+  float x[E], old[E], acc[E] = {};
   const uint32_t need = spoilt_columns<T, D>(to, j, g, lane, old);
-  load_row<T, D>(p.k, j, g, lane, k);
-  load_row<T, D>(p.v, j, g, lane, v);
-  for (int i0 = j; i0 < hi && !all_lost(acc, need); i0 += 4) {
+  load_row<T, D>(p.k, j, g, lane, x);
+  keep_row(buf, lane, x, p.scale_log2);
+  load_row<T, D>(p.v, j, g, lane, x);
+  keep_row(buf + D, lane, x, 1.f);
+  __syncwarp();
+  for (int first = j; first < hi && !all_lost(acc, need); first += 32) {
+    const int i = first + lane, count = min(32, hi - first);
     for (int h = g * group; h < (g + 1) * group; ++h) {
-      const float2* stat = p.stat + (int64_t)h * p.Np;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float q[E], d[E];
-        const int i = min(i0 + u, hi - 1);
-        load_row<T, D>(p.q, i, h, lane, q);
-        load_row<T, D>(p.dout, i, h, lane, d);
-        const float2 st = stat[i];
-        const float w = exp2f(dot(q, k) * p.scale_log2 + st.x);
-        const float ds = w * (dot(d, v) + st.y);
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = i0 + u < hi ? fmaf(want_dk ? ds : w, want_dk ? q[e] : d[e], acc[e]) : acc[e];
+      float w = 0.f;
+      if (lane < count) {
+        const float2 st = p.stat[(int64_t)h * p.Np + i];
+        w = exp2f(dot_row<T, D>(p.q, i, h, buf) + st.x);
+        if (want_dk) w *= dot_row<T, D>(p.dout, i, h, buf + D) + st.y;
       }
+      add_rows<T, D>(want_dk ? p.q : p.dout, first, 1, count, h, w, lane, acc);
     }
   }
   const float f = (want_dk ? p.scale : 1.f) * power_of_2(-(int)kUp<T>);  // stat raised the weights
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = (need >> e) & 1u ? acc[e] * f : old[e];
   store_row<T, D>(to, j, g, lane, acc);
+  __syncwarp();
 }
 
 // the largest of the values (none negative) of a warp's lanes that have the same seq
@@ -506,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
     *abort_flag = 1;
     if (status) atomicCAS(status, 0, code);
   };
-  auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, kBudgetNs, abort_flag, status); };
+  auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, p.wait_ns, abort_flag, status); };
   auto item_of = [&](int slot) {
     FwdItem I = item_rows(ring[slot * 4], gridDim.x, p);
     I.lo[0] = ring[slot * 4 + 1];
@@ -685,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
         } else if ((++spin & 255u) == 0) {
           if (spin == 256) since = globaltimer_ns();
           if (*abort_flag || (status && *reinterpret_cast<const volatile int*>(status)) ||
-              globaltimer_ns() - since > kBudgetNs) {
+              globaltimer_ns() - since > p.wait_ns) {
             ok = false;
             break;
           }
@@ -742,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
     } now, next;
     auto fetch = [&](int n, Work& w) -> bool {
       const int slot = n & 1;
-      if (!mbar_wait_warp(&item_full[slot], (n >> 1) & 1, kBudgetNs, abort_flag, status)) {
+      if (!mbar_wait_warp(&item_full[slot], (n >> 1) & 1, p.wait_ns, abort_flag, status)) {
         fail(kErrTimeoutEpilogue);
         return false;
       }
@@ -773,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
       for (int t = t_lo; t < t_hi; ++t) {
         const int set = t & 1;
         const uint32_t set_base = lane_base + set * 64;
-        if (!mbar_wait_warp(&s_full[2 * x + set], (sc >> set) & 1, kBudgetNs, abort_flag, status)) {
+        if (!mbar_wait_warp(&s_full[2 * x + set], (sc >> set) & 1, p.wait_ns, abort_flag, status)) {
           fail(kErrTimeoutEpilogue);
           ok = false;
           break;
@@ -836,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
               l *= alpha;
               m_ref = mx;
             }
-            if (!mbar_wait_warp(&pv_done[x], (pv - 1) & 1, kBudgetNs, abort_flag, status)) {
+            if (!mbar_wait_warp(&pv_done[x], (pv - 1) & 1, p.wait_ns, abort_flag, status)) {
               fail(kErrTimeoutEpilogue);
               ok = false;
               break;
@@ -872,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
       more = ok && fetch(n + 1, next);
       if (!more) break;
       if (t_hi <= t_lo) continue;
-      if (!mbar_wait_warp(&o_done[x], oc & 1, kBudgetNs, abort_flag, status)) {
+      if (!mbar_wait_warp(&o_done[x], oc & 1, p.wait_ns, abort_flag, status)) {
         fail(kErrTimeoutEpilogue);
         break;
       }
@@ -942,7 +968,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
       while (redo) {
         const int b = __ffs((int)redo) - 1;
         redo &= redo - 1;
-        fwd_row<T, D>(p, i - lane + b, h, lane);
+        fwd_row<T, D>(p, i - lane + b, h, lane, reinterpret_cast<float*>(out_buf));
       }
     }
     if (lane == 0) out_wait_done();
@@ -1363,7 +1389,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_tc_kernel(const __grid_constan
         const int b = __ffs((int)redo) - 1;
         redo &= redo - 1;
         const float2 st = make_float2(__shfl_sync(0xffffffffu, stat.x, b), __shfl_sync(0xffffffffu, stat.y, b));
-        dq_row<T, D>(p, i - lane + b, h, half, lane, st);
+        dq_row<T, D>(p, i - lane + b, h, half, lane, st, reinterpret_cast<float*>(smem + C::oK + (warp - 4) * kOutBytes));
       }
     } else if (ok) {
       fail(kErrTimeoutEpilogue);
@@ -1659,7 +1685,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_tc_kernel(const __grid_consta
       while (redo) {
         const int b = __ffs((int)redo) - 1;
         redo &= redo - 1;
-        dkv_row<T, D>(p, j - lane + b, kvh, half, lane);
+        dkv_row<T, D>(p, j - lane + b, kvh, half, lane, reinterpret_cast<float*>(smem + C::oQ + (warp - 4) * kOutBytes));
       }
     } else if (ok) {
       fail(kErrTimeoutEpilogue);
@@ -1745,6 +1771,8 @@ PackedParams common_params(const char* what, const torch::Tensor& q, const torch
   p.q = rows_of(q);
   p.k = rows_of(k);
   p.v = rows_of(v);
+  // up to 32 rows of a warp by themselves: 7 us per key in all (200,000 keys, 128 wide), and three times that allowed
+  p.wait_ns = kBudgetNs + 20000ull * p.window;
   p.start = start.data_ptr<int>();
   p.end = end.data_ptr<int>();
   return p;

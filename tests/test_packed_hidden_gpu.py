@@ -106,3 +106,21 @@ def test_no_numbers_throughout_cost_little(cuda, what):
         assert out[:, :, 3].isnan().all() and torch.isfinite(out[:, :, 4:]).all()
     # 30 ms without them; row by row it would be the order of a second
     assert a.elapsed_time(b) < 200, a.elapsed_time(b)
+
+
+def test_rows_by_themselves_in_a_very_long_sequence(cuda):
+    """Some rows at the end of 400,060 are computed alone, which takes seconds: no other warp's wait runs out."""
+    packed, check_status = _ops()
+    L, H, KV, D = 400_060, 2, 1, 64  # 60 rows share their tile with the next sequence
+    n = L + 100
+    q, k, v, _ = _inputs(n, H, KV, D, torch.bfloat16)
+    start, end = (t.cuda() for t in spans([L, 100], n))
+    want = packed.attention_fwd(q, k, v, start, end)
+    v[L, 0, 3] = math.nan
+    out, lse = packed.attention_fwd(q, k, v, start, end)
+    torch.cuda.synchronize()
+    assert check_status() == 0
+    # computed in another order, in fp32: both are within a rounding of P and of the result
+    near = 2.0 ** -8 * want[0][L - 200:L].float().abs() + 2.0 ** -8 * v[:L].float().abs().mean()
+    assert ((out[L - 200:L].float() - want[0][L - 200:L].float()).abs() <= near).all()
+    assert torch.equal(lse[:, :L], want[1][:, :L]) and torch.equal(out[:L - 1000], want[0][:L - 1000])
