@@ -144,7 +144,8 @@ template <typename T, int D>
 __device__ __noinline__ int2 odd_rows(const Rows& r, int h0, int h1, int lo, int hi, int lane) {
   constexpr uint32_t kExp = Half16<T>::kFormat ? 0x7f80u : 0x7c00u;
   int first = INT_MAX, last = -1;
-  for (int i = lo + lane; i < hi; i += 32) {
+  // lo may be any number where the spans are none; hi is a row
+  for (int i = lo < hi ? lo + lane : hi; i < hi; i += 32) {
     bool odd = false;
     for (int h = h0; h < h1; ++h) {
       const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(r.p) + (int64_t)i * r.row + h * r.head);
