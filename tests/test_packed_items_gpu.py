@@ -145,3 +145,27 @@ def test_bad_spans_write_nothing_outside(cuda, n, D, dt, window, kind):
         assert (buf.view(-1)[:before] == 7.0).all() and (buf.view(-1)[before + count:] == 7.0).all()
     if kind == "none":
         assert all((t == 7.0).all() for t in (out, lse, dq, dk, dv))
+
+
+@pytest.mark.parametrize("D,dt", [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("lengths,tail", [([500, 1, 200], 3), ([1], 0), ([130], 0)])
+def test_outputs_of_any_layout(cuda, lengths, tail, D, dt):
+    """Outputs stored head by head, or between other columns: the bits of dense ones, and nothing around them written."""
+    packed, check_status = _ops()
+    H, KV, n = 4, 2, sum(lengths) + tail
+    g = torch.Generator(device="cuda").manual_seed(n)
+    r = lambda h: torch.randn(n, h, D, generator=g, device="cuda").to(dt)  # noqa: E731
+    q, k, v, do = r(H), r(KV), r(KV), r(H)
+    start, end = (t.cuda() for t in spans(lengths, n))
+    want = packed.attention_fwd(q, k, v, start, end)
+    want += packed.attention_bwd(q, k, v, *want, do, start, end)
+    whole = lambda *s: torch.full(s, 7.0, device="cuda").to(dt)  # noqa: E731
+    for make in (lambda h: (b := whole(h, n, D), b.transpose(0, 1)), lambda h: (b := whole(n, 2 * h + 1, D + 16), b[:, 1:h + 1, 8:D + 8])):
+        (ob, out), (qb, dq), (kb, dk), (vb, dv) = make(H), make(H), make(KV), make(KV)
+        packed.attention_fwd(q, k, v, start, end, out=out)
+        packed.attention_bwd(q, k, v, want[0], want[1], do, start, end, dq=dq, dk=dk, dv=dv)
+        for buf, view, right in ((ob, out, want[0]), (qb, dq, want[2]), (kb, dk, want[3]), (vb, dv, want[4])):
+            assert torch.equal(view[:n - tail], right[:n - tail])
+            view[:n - tail] = 7.0
+            assert (buf == 7.0).all()
+    assert check_status() == 0
