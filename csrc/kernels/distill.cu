@@ -397,7 +397,8 @@ __global__ void __launch_bounds__(NT + 32 * TW + 32, MINB) distill_kernel(const 
           for (int i = 0; i < p.K; ++i)
             if (s_id[i] == id) q = s_q[i];
         }
-        float g = f32x2_split(dense(l, l, f)).x - f.ct * q;
+        float g = f32x2_split(dense(l, l, f)).x;
+        if (f.ct != 0.f) g -= f.ct * q;  // without weight the teacher may hold anything
         if (MODE != kSoft && id == y) g -= f.ch;
         G[id] = Vec<T>::round(g * f32x2_split(slope(l, l)).x);
       }

@@ -129,3 +129,15 @@ def test_a_bad_id_costs_its_own_entry_alone(cuda, M, V, dt, t, alpha):
         _, rows, grad = op(z, ids, u, y, cap=15.0, temperature=t, alpha=alpha, scale=1.0)
         assert ((rows.double() - r).abs() <= rt).all() and ((grad.double() - g).abs() <= gt).all()
     assert check_status() == BAD_INDEX
+
+
+@pytest.mark.parametrize("V", [1000, 70_000])
+def test_a_teacher_of_no_weight_is_not_read_into_the_result(cuda, V):
+    """alpha = 0: loss and gradient are those of the hard labels, whatever the teacher's logits hold."""
+    op, check_status = _op()
+    z, ids, u, y = inputs(50, V, 8, torch.float32, 15.0, seed=2)
+    want = op(z, ids, u, y, alpha=0.0)
+    for what in (math.nan, math.inf, -math.inf):
+        got = op(z, ids, torch.full_like(u, what), y, alpha=0.0)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert torch.isfinite(want[2]).all() and check_status() == 0
