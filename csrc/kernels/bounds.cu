@@ -53,7 +53,8 @@ __global__ void __launch_bounds__(kOffThreads) bounds_offsets_kernel(const int* 
 // a running maximum of positions and the next BOS behind it a running minimum from the other side (warp
 // shuffles, then the 8 warps' results); the tile's first tokens and its last ones look for theirs in the
 // neighbouring tiles, a block-wide step of 2048 tokens at a time until one is found, which takes one step or
-// two where documents are shorter than that.
+// two where documents are shorter than that. A row without any BOS costs every tile a walk over all the others (2^18
+// tokens: up to 127 steps, one after the other).
 constexpr int kIdThreads = 256, kIdPer = 8, kIdTile = kIdThreads * kIdPer;
 
 __device__ __forceinline__ int block_max(int v, int* red) {
@@ -171,7 +172,8 @@ std::tuple<torch::Tensor, torch::Tensor> bounds_from_ids(const torch::Tensor& id
   TORCH_CHECK_VALUE(ids.scalar_type() == at::kInt && ids.dim() == 2 && (ids.size(1) <= 1 || ids.stride(1) == 1),
                     "bounds_from_ids: ids must be int32 [B, T] with contiguous rows");
   const int64_t B = ids.size(0), T = ids.size(1), rows = B * T;
-  TORCH_CHECK_VALUE(rows < (int64_t(1) << 31), "bounds_from_ids: too many tokens");
+  // the limit of the attention; positions and the tile behind them stay below 2^31
+  TORCH_CHECK_VALUE(rows < (int64_t(1) << 30), "bounds_from_ids: too many tokens");
   TORCH_CHECK_VALUE(bos >= INT32_MIN && bos <= INT32_MAX, "bounds_from_ids: bos is not an int32");
   torch::Tensor start = bounds_out(start_out, rows, ids, "start"), end = bounds_out(end_out, rows, ids, "end");
   check_output("bounds_from_ids", {"start", &start}, {{"end", &end}, {"ids", &ids}});
