@@ -81,6 +81,14 @@ template <typename T>
 constexpr bool kScaled = Half16<T>::kFormat == 0;
 template <typename T>
 constexpr float kUp = kScaled<T> ? 14.f : 0.f;
+// The forward's P is exp2(x - m + kRaise) with m the running maximum, which is replaced once it is exceeded by more than
+// kGrow in log2 units: rarely, with kGrow far above what the maximum of a block's scores usually gains on the first
+// block's. In fp16 P is then at most 2^15 and normal down to 2^-25 of the row's largest weight (with m alone and 2^8
+// of room weights below 2^-14 lost bits, and those below 2^-25, as beside one key that takes nearly all, vanished).
+template <typename T>
+constexpr float kRaise = kScaled<T> ? 11.f : 0.f;
+template <typename T>
+constexpr float kGrow = kScaled<T> ? 4.f : 8.f;
 __device__ __forceinline__ float power_of_2(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ int up_for(float b) {
   const int e = (__float_as_int(b) >> 23) - 127;  // b < 2^(e + 1)
@@ -350,21 +358,22 @@ __global__ void __launch_bounds__(kNormThreads) v_most_kernel(const __grid_const
 //   warps 1, 2 issue the MMAs of tile A and of B, by blocks of 64 keys with two score sets (set s = t % 2): S_X = Q_X K_t^T
 //              -> TMEM [256X + 64s, +64) fp32; P_X, written there by the softmax warps as 16-bit pairs over S_X, is
 //              the A operand of O_X += P_X V_t -> TMEM [256X + 128, +D). Order: PV_X(t), S_X(t+2), so the scores of
-//              block t + 1 stand ready while t's softmax runs, and neither waits for the other. One thread for both
+//              block t + 1 stand ready while t's softmax runs. One thread for both
 //              tiles took 600 to 1000 cycles for a block's twelve MMAs, its waits and commits, twice what they run;
 //   warp 3     loads the Q tiles, one lane each;
 //   warps 4-11 softmax, one query row per thread (4-7 tile A, 8-11 tile B), and the output through shared memory.
 // The two tiles meet only in the K and V rings (a slot is free when both have passed it), so one may be in its next
-// item while the other finishes: with short sequences an item is few blocks, and what it costs to start and
-// to end one (loads, output) hides behind the other tile's work.
-// P is at most 2^8 (the running maximum is only replaced when it grows by more than that) and is rounded to 16
-// bits for the product (half a step, relative); the row sum l adds the unrounded fp32 values, the maximum, l and
-// O stay in fp32.
+// item while the other finishes. What an item costs to start and to end (loads, output) hides behind the other tile's
+// work only where their blocks differ: two heads over the same rows have the same ones and start and end together,
+// and two row tiles' differ by two or so; with short sequences, where an item is few blocks, most of it lies open.
+// P is rounded to 16 bits for the product (half a step, relative to each weight, see kRaise); the row sum l adds the
+// unrounded fp32 values, the maximum, l and O stay in fp32.
 // Bounds: 4 D operations per pair on the tensor core, one exponential per pair (16 per SM and cycle, as long as the
 // pair's products at D = 128), and for the 64-key score products 6 KB of shared memory per 128 x 64 x 16 step. On
-// B200: one prompt of 16384 rows, 8 heads of 128 on 2, 466 us (1179 TFLOP/s; with 128-key blocks and one score set
-// 482 us, and 148 instead of 113 us in the next case); 65536 rows in documents of 512 on average, window 1024,
-// 4 x 128, 113 us (2.4 TB/s; an item's start, end and masks weigh as much as its nine blocks).
+// B200, several inputs in turn: one prompt of 16384 rows, 8 heads of 128 on 2, 537 us (1024 TFLOP/s); 65536 rows in
+// documents of 512 on average, window 1024, 4 x 128, 121 us (2.2 TB/s; an item's start, end and masks weigh as much as
+// its nine blocks). 32 rows of 2048, 4 x 128: 163 us, 193 with the fixed-length kernel of attention_tc.cu. On one input
+// over and over 128-key blocks with one score set took 482 us instead of 466, and 148 instead of 113 us.
 constexpr uint64_t kBudgetNs = 2000000000ull, kDrainNs = 100000000ull;
 constexpr int BT = 128;  // rows of a query tile (forward, dQ), keys of a tile (dK/dV)
 constexpr int BB = 64;   // keys (forward, dQ) or queries (dK/dV) of a block
@@ -809,7 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
         tc_fence_after();
         const int kx = key.x - t * BB, ky = key.y - t * BB;  // the row sees the keys [kx, ky) of the block
         // P = exp2(S scale - m) with the maximum so far: one pass, in which the block's own maximum is found beside
-        // the exponentials. Only where that exceeds the old one by more than 2^8 are the scores read again and
+        // the exponentials. Only where that exceeds the old one by more than kGrow are the scores read again and
         // the exponentials taken anew (an item's first block finds its maximum beforehand). P replaces S once
         // it stands.
         uint32_t pk[32];
@@ -835,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
           mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * p.scale_log2;
           if (first) m_ref = mx;
           const float mref = m_ref == -INFINITY ? 0.f : m_ref;
-          const uint64_t sc2 = f32x2(p.scale_log2, p.scale_log2), nm2 = f32x2(-mref, -mref);
+          const uint64_t sc2 = f32x2(p.scale_log2, p.scale_log2), nm2 = f32x2(kRaise<T> - mref, kRaise<T> - mref);
           uint64_t l2[2] = {0, 0};
 #pragma unroll
           for (int e = 0; e < BB; e += 2) {
@@ -855,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
           // The rescale is decided per row, but tcgen05.ld/st are warp-collective: the warp rescales together
           // when any of its rows needs it, the others by 1, and after the last block's product with V (the one
           // before that has completed: it was issued before these scores).
-          const bool mine = mx > m_ref + 8.f;
+          const bool mine = mx > m_ref + kGrow<T>;
           if (__any_sync(0xffffffffu, mine)) {
             float alpha = 1.f;
             if (mine) {
@@ -948,7 +957,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
         }
         __syncwarp();
       }
-      if (real) p.lse[(int64_t)h * p.N + i] = (m_ref + log2f(l)) * kLn2;
+      if (real) p.lse[(int64_t)h * p.N + i] = (m_ref - kRaise<T> + log2f(l)) * kLn2;
       // rows that are no numbers although their scores are, and whose tiles hold foreign keys that were not cleared, or
       // hidden keys of the row's own sequence that are no numbers
       bool again = real && odd != 0.f && l == l;
@@ -989,7 +998,8 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_tc_kernel(const __grid_consta
 // 64 keys or queries at a time, 384 threads: warp 0 loads (TMA), warp 1 issues the MMAs, warps 4-7 and 8-11 turn
 // scores into P and dS, one tile row per thread, the two groups taking the blocks in turn: while one group
 // loads, computes and stores, the other's block goes through the tensor core. P and dS are rounded to 16 bits
-// for their products (half a step, relative to each entry); everything else is fp32. They are written over the
+// for their products (half a step, relative to each entry: in fp16 after a power of two, see kUp, which with its bounds
+// makes 65536 rows' forward and backward 611 us instead of 556); everything else is fp32. They are written over the
 // scores that they came from. On B200, 65536 rows in documents of 512 on average, 4 x 128 heads: dQ 0.20 ms, dK/dV
 // 0.26 ms, where a block's start and end lie open between two tiles of an SM; 8192 rows, 16 heads of 128 on 4: dQ
 // 0.36 ms (0.6 of the tensor core's cycles), dK/dV 0.53 ms, bound by the shared memory that its products read (128
@@ -1045,9 +1055,10 @@ __device__ __forceinline__ bool store_cols(uint32_t taddr, float f, const Rows& 
 // K and V from shared memory. The kernel also computes delta = rowsum(dO o O) and leaves lse and delta of each row
 // for the dK/dV kernel. Two roundings are undone here, since with dS rounded once and O's rounding in delta, dQ
 // and dK came out 1.5 to 1.6 times as far from 64 bits as one rounding of the result alone: the tile's last two
-// blocks, where the rows of few keys and large weights have all of theirs, take dS in two 16-bit parts, and the
-// delta that goes to dK/dV is the sum of P dP itself, in fp32, which this kernel has at hand. (Both parts in every
-// block: 219 instead of 184 us over 65536 packed tokens.)
+// blocks take dS in two 16-bit parts, and the delta that goes to dK/dV is the sum of P dP itself, in fp32, which this
+// kernel has at hand. The last two blocks are a compromise: rows of few keys and large weights have theirs there,
+// unless their document starts a few rows before the tile does. (Both parts in every block: 219 instead of 184 us
+// over 65536 packed tokens.)
 template <int D>
 struct DqCfg {
   static constexpr int kTile = BB * D * 2;

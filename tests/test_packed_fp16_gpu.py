@@ -105,3 +105,28 @@ def test_large_gradients_do_not_overflow(cuda, lengths):
     r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
     q, k, v = (0.05 * r(n, H, D)).half(), (0.05 * r(n, H, D)).half(), (20 * r(n, H, D)).half()
     check(packed, q, k, v, (1500 * r(n, H, D)).half(), lengths)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("below", [13.7, 17.3, 20.7, 24.6])
+def test_weights_far_below_the_largest(cuda, D, below):
+    """One key that takes nearly all of the weight, and thousands of others with 2^-below of it each, whose values are the
+    only ones: the result is their sum, each weight rounded once."""
+    packed, check_status = _ops()
+    n, scale = 9000, 1 / math.sqrt(D)
+    q = torch.ones(n, 1, D, device="cuda").half()
+    k = torch.zeros(n, 1, D, device="cuda").half()
+    k[0] = below * math.log(2) / (scale * D)
+    v = torch.ones(n, 1, D, device="cuda").half()
+    v[0] = 0.0
+    start, end = (t.cuda() for t in spans([n], n))
+    out, lse = packed.attention_fwd(q, k, v, start, end)
+    torch.cuda.synchronize()
+    assert check_status() == 0
+    x = scale * D * float(k[0, 0, 0].double())
+    i = torch.arange(n, dtype=torch.float64, device="cuda")
+    want = i / (math.exp(x) + i)
+    # a weight's rounding and the result's, the score's fp32 error (2^-20 of it) and the sums'
+    tol = want * (2 * HALF_STEP + x * 2.0 ** -20 + 1e-4) + 2.0 ** -25
+    assert ((out[:, 0].double() - want[:, None]).abs() <= tol[:, None]).all()
+    assert ((lse[0].double() - torch.log(math.exp(x) + i)).abs() <= 1e-4).all()
