@@ -25,9 +25,11 @@
 // that is the exponential unit, 16 results per SM and cycle: a value that both passes need costs two of them. p
 // and P therefore come from one exponential where t is 1 (they are the same) or 2 (exp(x) is the square of
 // exp(x / 2), which doubles a relative error of 2^-22).
-// On B200: 8191 x 65536 bf16 413 us (5.2 TB/s, 0.80 of the measured copy); 32768 x 8192 bf16 with targets at t = 2
-// 306 us (3.5 TB/s; 22 instructions per logit, a row's fixed part among them, fill half of the issue slots). With
-// one block per row, no ring and no entries' warps it was 378 us there, and 690 us for the wide rows.
+// On B200: 8191 x 65536 bf16 408 us (5.3 TB/s, 0.80 of the measured copy); 32768 x 8192 bf16 with targets at t = 2
+// 302 us (3.6 TB/s; 22 instructions per logit, a row's fixed part among them, fill half of the issue slots, and a
+// barrier per row is among the leading stalls), at t = 1.5 415 us (four exponentials per logit), the loss alone 153
+// us, the same rows in fp32 607 us. With one block per row, no ring and no entries' warps it was 378 us at t = 2, and
+// 690 us for the wide rows.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
