@@ -229,7 +229,10 @@ class FusedGPTEngine:
 
     def _teacher_head(self, tg: torch.Tensor, b: dict, scale: float, teacher: Teacher):
         """lm_head + softcap 15, then the loss against the teacher's top logits; G becomes its gradient with respect
-        to the scores before the softcap (the logits do reach memory here: the teacher's columns are read from them)."""
+        to the scores before the softcap (the logits do reach memory here: the teacher's columns are read from them).
+        They are bf16, in the buffer that the gradient replaces: a logit of 8 to 15 is off by up to 1/32, and with it
+        the loss of both parts, where the head without a teacher takes fp32 accumulators; the softcap's slope
+        1 - (l / 15)^2 is off by up to 1/240, so next to the cap, where it is as small, it is mostly rounding."""
         M = tg.numel()
         gemm.matmul(b["xf"], self.shadows["lmHead"].t(), out=b["G"], epi=gemm.SOFTCAP, alpha=1.0 / 15.0, beta=15.0)
         loss, _, _ = distill_topk(b["G"], teacher.ids.reshape(M, -1), teacher.logits.reshape(M, -1), tg, cap=15.0,
