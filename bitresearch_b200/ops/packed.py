@@ -7,7 +7,8 @@ which each document starts with BOS, are made once per batch, and serve the forw
 
 Row ``i`` sees the rows ``j`` of its sequence with ``i - window < j <= i`` (``window=0``: all up to ``i``).
 What a row does not see (other sequences, later rows, rows outside its window, padding rows) does not reach its results,
-values that are no numbers included, nor do queries that do not see a key reach that key's gradients; rows of no
+values that are no numbers included, nor do queries that do not see a key reach that key's gradients (a value that is no
+number because of what its row does see may be infinite or NaN, whichever comes first); rows of no
 sequence are left as they were in every output (zero in one that the call makes).
 Spans must be those of sequences that follow one another; any other contents give wrong values but read and
 write no row outside the tensors.

@@ -108,6 +108,42 @@ def test_no_numbers_throughout_cost_little(cuda, what):
     assert a.elapsed_time(b) < 200, a.elapsed_time(b)
 
 
+@pytest.mark.parametrize("what", ["v", "v column", "do", "do column"])
+def test_infinities_throughout_cost_little(cuda, what):
+    """As overflowed half-precision values are: the computation of a row alone ends at the first infinity too."""
+    packed, check_status = _ops()
+    n, H, KV, D = 40_000, 4, 2, 128
+    q, k, v, do = _inputs(n, H, KV, D, torch.float16)
+    start, end = (t.cuda() for t in spans([n], n))
+    if what == "v":
+        v[100:] = math.inf
+    elif what == "v column":
+        v[:, :, 3] = -math.inf
+    elif what == "do":
+        do[:] = math.inf
+    else:
+        do[:, :, 5] = math.inf
+
+    def run():
+        out, lse = packed.attention_fwd(q, k, v, start, end)
+        return out, *packed.attention_bwd(q, k, v, out, lse, do, start, end)
+
+    run()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    out, dq, dk, dv = run()
+    b.record()
+    torch.cuda.synchronize()
+    assert check_status() == 0
+    if what == "v":
+        assert torch.isfinite(out[:100]).all() and not torch.isfinite(out[100:]).any()
+    elif what == "v column":
+        assert not torch.isfinite(out[:, :, 3]).any() and torch.isfinite(out[:, :, 4:]).all()
+    elif what == "do column":
+        assert not torch.isfinite(dv[:, :, 5]).any() and torch.isfinite(dv[:, :, 6:]).all()
+    assert a.elapsed_time(b) < 200, a.elapsed_time(b)
+
+
 def test_rows_by_themselves_in_a_very_long_sequence(cuda):
     """Some rows at the end of 400,060 are computed alone, which takes seconds: no other warp's wait runs out."""
     packed, check_status = _ops()
