@@ -40,7 +40,7 @@ def bounds_from_offsets(offsets: torch.Tensor, rows: int, start: torch.Tensor | 
 def bounds_from_ids(ids: torch.Tensor, bos: int, start: torch.Tensor | None = None,
                     end: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``(start, end)`` of the ``B * T`` rows of ``ids`` (int32 ``[B, T]``): a sequence starts at every ``bos`` and
-    at the first token of each of the ``B`` rows of ids."""
+    at the first token of each of the ``B`` rows of ids. Fewer than 2^30 tokens."""
     return ext().bounds_from_ids(ids, bos, start, end)
 
 

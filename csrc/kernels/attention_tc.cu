@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(320, 1)
 
   const int n_items = ((p.T + 2 * BQ - 1) / (2 * BQ)) * p.H * p.B;
   const int warp = warp_id();
-  if (device_failed(p.status)) {
+  if (__syncthreads_or(device_failed(p.status))) {  // all threads or none: the word may change meanwhile
     if (threadIdx.x == 0) fwd_sched_exit();
     return;
   }
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(320, 1)
   const int kb_hi = min(q0 + BQ - 1, p.T - 1) / BK64;
   const int nkv = kb_hi - kb_lo + 1;
   const int warp = warp_id();
-  if (device_failed(p.status)) return;
+  if (__syncthreads_or(device_failed(p.status))) return;  // all threads or none
   if (threadIdx.x == 0) {
     mbar_init(q_full, 256);  // every softmax thread has stored its Q or dO row in TMEM
     for (int i = 0; i < DQ_STAGES; ++i) {
@@ -842,7 +842,7 @@ __global__ void __launch_bounds__(320, 1)
   const int nq = qb_hi - qb_lo + 1;
   const int iters = nq * group;
   const int warp = warp_id();
-  if (device_failed(p.status)) return;
+  if (__syncthreads_or(device_failed(p.status))) return;  // all threads or none
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
     for (int i = 0; i < DK_STAGES; ++i) {

@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(GemmCfg<BN, AUX, CG, epi_warps(EPI, AUX, CG)>:
 
   // an early return is for single CTAs only: a pair must reach its cluster barriers together
   if constexpr (CG == 1) {
-    if (device_failed(p.status)) return;
+    if (__syncthreads_or(device_failed(p.status))) return;  // all threads or none: the word may change meanwhile
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
